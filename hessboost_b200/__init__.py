@@ -5,7 +5,9 @@ whose entry points mirror hessboost's ``HistogramBackend`` / ``RowEngine``
 backend seam (``src/tree/hist/mod.rs:73-295``) and its GPU prediction model.
 This module binds it with ctypes and offers the reference's user-level verbs
 on top: cuts and binning of a dense matrix, ``train`` of a single-output
-squared-error or logistic model, and batch ``predict_margin``.
+squared-error or logistic model, and batch ``predict_margin``. The operators
+of an embedding head over the same binned matrix are in ``head`` (torch
+tensors; import it by name).
 
 There is no CPU fallback: every computing call goes to the CUDA library, and
 importing a missing library raises.
@@ -225,6 +227,7 @@ assert NODE_DTYPE.itemsize == ctypes.sizeof(TreeNode) == 40
 _P = ctypes.POINTER
 _u8p, _u32p, _u64p, _f32p = _P(ctypes.c_uint8), _P(ctypes.c_uint32), _P(ctypes.c_uint64), _P(ctypes.c_float)
 _vp, _i32p = ctypes.c_void_p, _P(ctypes.c_int32)
+_i32, _u32, _u64, _f32 = ctypes.c_int32, ctypes.c_uint32, ctypes.c_uint64, ctypes.c_float
 SIGNATURES = {
     "hb_engine_create": [ctypes.c_int32, _P(_vp)],
     "hb_engine_destroy": [_vp],
@@ -282,8 +285,27 @@ SIGNATURES = {
     "hb_probe_smem": [ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32,
                       ctypes.POINTER(ctypes.c_double)],
     "hb_peer_wait_probe": [ctypes.c_int32, ctypes.c_int32, _u64p, ctypes.POINTER(ctypes.c_double)],
+    # embedding-head operators (hessboost_b200/head.py)
+    "hb_head_last_error": [],
+    "hb_embed_forward": [_i32, _vp, _i32, _vp, _u64, _u64, _vp, _i32, _u64, _u32, _u64, _f32, _vp, _vp],
+    "hb_embed_backward_workspace": [_u64, _u64, _u64, _u32, _u64p],
+    "hb_embed_backward": [_i32, _vp, _i32, _vp, _u64, _u64, _vp, _i32, _u64, _u64, _u32, _f32, _vp, _vp, _u64,
+        _vp],
+    "hb_layer_norm_forward": [_i32, _vp, _i32, _u64, _u64, _u32, _vp, _vp, _i32, _f32, _vp, _vp, _vp, _vp],
+    "hb_layer_norm_backward_workspace": [_u64, _u32, _u64p],
+    "hb_layer_norm_backward": [_i32, _vp, _u64, _vp, _u64, _i32, _u64, _u32, _vp, _i32, _vp, _vp, _vp, _vp, _vp,
+        _vp, _u64, _vp],
+    "hb_linear_xent_forward_workspace": [_u64, _u32, _u64, _i32, _u64p],
+    "hb_linear_xent_forward": [_i32, _vp, _u64, _vp, _u64, _i32, _vp, _i32, _u64, _u32, _u64, _vp, _vp, _vp, _u64,
+        _vp],
+    "hb_linear_xent_backward_workspace": [_u64, _u32, _u64, _i32, _u64p],
+    "hb_linear_xent_backward": [_i32, _vp, _u64, _vp, _u64, _vp, _u64, _i32, _vp, _i32, _vp, _u64, _u32, _u64,
+        _vp, _vp, _vp, _u64, _vp],
+    "hb_grad_norm_workspace": [_i32, _vp, _u64p],
+    "hb_grad_norm": [_i32, _i32, _vp, _vp, _vp, _vp, _vp, _u64, _vp],
+    "hb_clip_grad_norm": [_i32, _i32, _vp, _vp, _vp, _vp, _f32, _vp, _vp, _u64, _vp],
 }
-_STRING_RESULT = ("hb_engine_last_error", "hb_sketch_last_error")
+_STRING_RESULT = ("hb_engine_last_error", "hb_sketch_last_error", "hb_head_last_error")
 
 _lib = None
 

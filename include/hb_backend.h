@@ -425,6 +425,108 @@ hb_status hb_engine_upload_csr(hb_engine* e, const uint64_t* indptr, const uint3
                                uint32_t max_bin, uint32_t* feature_offset, float* cut_values,
                                uint64_t cap, uint64_t* total);
 
+/* ---- embedding-head operators (no counterpart in the reference) ----------
+ * One training step of a differentiable head on the matrix's tokens (a row's
+ * global bins): embedding, layer norm, linear softmax cross entropy over any
+ * number of classes, gradient clipping.
+ *
+ * Unlike the calls above these take DEVICE memory of GPU `device`, strides
+ * in elements, and the caller's stream (a cudaStream_t; NULL: the default
+ * stream). They enqueue their kernels there and return without waiting;
+ * they allocate nothing, keep nothing between calls and put the calling
+ * thread's current device back. Where a call needs scratch, the matching
+ * *_workspace function gives the bytes, and the scratch must stay untouched
+ * until the stream has passed the call. Different calls may run at the same
+ * time if their workspaces and outputs do not overlap. Outputs must not
+ * overlap inputs unless said. Results do not change from run to run.
+ * HB_INVALID_ARGUMENT (the reason in hb_head_last_error) leaves everything
+ * untouched; HB_REFUSED means there is no such device. Sums, softmax
+ * statistics and norms are f32 or wider whatever the elements' type, and
+ * each output is rounded once. Sizes of 0 rows, cells or tensors are valid. */
+#define HB_F32 0  /* element types */
+#define HB_F16 1
+#define HB_BF16 2
+#define HB_I32 0  /* token and label types */
+#define HB_I64 1
+/* The reason for the calling thread's last failure of an hb_embed_*,
+ * hb_layer_norm_*, hb_linear_xent_*, hb_grad_norm or hb_clip_grad_norm call
+ * ("" after a success); valid until that thread's next such call. */
+const char* hb_head_last_error(void);
+
+/* out[n] = scale * sum over the cells c of row n of table[tokens[c]].
+ * Row n's cells are [row_ptr[n], row_ptr[n + 1]) (a CSR index's offsets,
+ * n_rows + 1 ascending values), or, with row_ptr NULL, n_cells / n_rows
+ * consecutive ones each (1: a plain lookup). A token outside [0, n_tokens)
+ * is a missing cell and contributes nothing; a row without cells is 0.
+ * table: n_tokens x width, out: n_rows x width (contiguous), both of
+ * `dtype`. */
+hb_status hb_embed_forward(int32_t device, const void* tokens, int32_t token_type, const int64_t* row_ptr,
+                           uint64_t n_rows, uint64_t n_cells, const void* table, int32_t dtype,
+                           uint64_t n_tokens, uint32_t width, uint64_t table_stride, float scale,
+                           void* out, void* stream);
+/* The table's gradient: dtable[v] = scale * sum over the cells c whose token
+ * is v of grad[row of c], in cell order; every row of dtable (n_tokens x
+ * width, contiguous) is written. grad_stride 0: one row for all. */
+hb_status hb_embed_backward_workspace(uint64_t n_rows, uint64_t n_cells, uint64_t n_tokens, uint32_t width,
+                                      uint64_t* bytes);
+hb_status hb_embed_backward(int32_t device, const void* tokens, int32_t token_type, const int64_t* row_ptr,
+                            uint64_t n_rows, uint64_t n_cells, const void* grad, int32_t dtype,
+                            uint64_t grad_stride, uint64_t n_tokens, uint32_t width, float scale,
+                            void* dtable, void* workspace, uint64_t workspace_bytes, void* stream);
+
+/* y = (x - mean) rstd weight + bias over each row's `width` elements, rstd =
+ * 1 / sqrt(variance + eps); mean and rstd (n_rows f32 each) are kept for the
+ * backward pass. weight and bias may be NULL (1 and 0); param_type is x's
+ * type or HB_F32. y is contiguous. */
+hb_status hb_layer_norm_forward(int32_t device, const void* x, int32_t dtype, uint64_t x_stride,
+                                uint64_t n_rows, uint32_t width, const void* weight, const void* bias,
+                                int32_t param_type, float eps, void* y, float* mean, float* rstd,
+                                void* stream);
+/* dx of x's type (contiguous), dweight and dbias of param_type (each may be
+ * NULL: not wanted), summed over the rows in a fixed order. */
+hb_status hb_layer_norm_backward_workspace(uint64_t n_rows, uint32_t width, uint64_t* bytes);
+hb_status hb_layer_norm_backward(int32_t device, const void* dy, uint64_t dy_stride, const void* x,
+                                 uint64_t x_stride, int32_t dtype, uint64_t n_rows, uint32_t width,
+                                 const void* weight, int32_t param_type, const float* mean,
+                                 const float* rstd, void* dx, void* dweight, void* dbias,
+                                 void* workspace, uint64_t workspace_bytes, void* stream);
+
+/* loss[n] = lse[n] - z[n][label], lse[n] = log(sum over the classes of
+ * exp(z[n])), z = x w^T: x n_rows x width, w n_classes x width, both f32 or
+ * both bf16. The logits are never kept. A label outside [0, n_classes) is a
+ * row without a label: its loss is 0 (its lse is still written). */
+hb_status hb_linear_xent_forward_workspace(uint64_t n_rows, uint32_t width, uint64_t n_classes,
+                                           int32_t dtype, uint64_t* bytes);
+hb_status hb_linear_xent_forward(int32_t device, const void* x, uint64_t x_stride, const void* w,
+                                 uint64_t w_stride, int32_t dtype, const void* labels, int32_t label_type,
+                                 uint64_t n_rows, uint32_t width, uint64_t n_classes, float* loss,
+                                 float* lse, void* workspace, uint64_t workspace_bytes, void* stream);
+/* dx and dw (contiguous) of sum over n of dloss[n * dloss_stride] loss[n]
+ * (dloss_stride 0: one factor for every row); lse from the forward pass. The
+ * logits are computed again, a piece of the classes at a time. Rows without
+ * a label get 0 and add nothing. */
+hb_status hb_linear_xent_backward_workspace(uint64_t n_rows, uint32_t width, uint64_t n_classes,
+                                            int32_t dtype, uint64_t* bytes);
+hb_status hb_linear_xent_backward(int32_t device, const float* dloss, uint64_t dloss_stride, const void* x,
+                                  uint64_t x_stride, const void* w, uint64_t w_stride, int32_t dtype,
+                                  const void* labels, int32_t label_type, const float* lse,
+                                  uint64_t n_rows, uint32_t width, uint64_t n_classes, void* dx, void* dw,
+                                  void* workspace, uint64_t workspace_bytes, void* stream);
+
+/* *norm (device, f32) = the 2-norm of all the tensors' elements together.
+ * `tensors`, `sizes` (elements) and `dtypes` are host arrays, read before
+ * the call returns; tensors[i] is contiguous device memory. */
+hb_status hb_grad_norm_workspace(int32_t n_tensors, const uint64_t* sizes, uint64_t* bytes);
+hb_status hb_grad_norm(int32_t device, int32_t n_tensors, const void* const* tensors, const uint64_t* sizes,
+                       const int32_t* dtypes, float* norm, void* workspace, uint64_t workspace_bytes,
+                       void* stream);
+/* hb_grad_norm, then outs[i] = tensors[i] * min(1, max_norm / (*norm +
+ * 1e-6)), each of its tensor's type; outs[i] may be tensors[i]. A norm that
+ * is not finite shows in *norm and passes into the outputs. */
+hb_status hb_clip_grad_norm(int32_t device, int32_t n_tensors, const void* const* tensors, void* const* outs,
+                            const uint64_t* sizes, const int32_t* dtypes, float max_norm, float* norm,
+                            void* workspace, uint64_t workspace_bytes, void* stream);
+
 /* ---- native binary model files (BoostedModel::encode/decode,
  * src/model/native.rs, src/model/container.rs) ---------------------------
  * XXH64 (seed 0) of `len` bytes: the checksum that closes a native model

@@ -159,4 +159,43 @@ extern "C" {
                          lane_ops_per_clk: *mut f64) -> hb_status;
     pub fn hb_engine_inject_fault(e: *mut hb_engine, after_calls: i32) -> hb_status;
     pub fn hb_peer_wait_probe(device: i32, timeout_ms: i32, status: *mut u64, waited_ms: *mut f64) -> hb_status;
+    // embedding-head operators: device memory and a cudaStream_t
+    pub fn hb_head_last_error() -> *const c_char;
+    pub fn hb_embed_forward(device: i32, tokens: *const c_void, token_type: i32, row_ptr: *const
+        i64, n_rows: u64, n_cells: u64, table: *const c_void, dtype: i32, n_tokens: u64, width: u32,
+        table_stride: u64, scale: f32, out: *mut c_void, stream: *mut c_void) -> hb_status;
+    pub fn hb_embed_backward_workspace(n_rows: u64, n_cells: u64, n_tokens: u64, width: u32, bytes:
+        *mut u64) -> hb_status;
+    pub fn hb_embed_backward(device: i32, tokens: *const c_void, token_type: i32, row_ptr: *const
+        i64, n_rows: u64, n_cells: u64, grad: *const c_void, dtype: i32, grad_stride: u64, n_tokens:
+        u64, width: u32, scale: f32, dtable: *mut c_void, workspace: *mut c_void, workspace_bytes:
+        u64, stream: *mut c_void) -> hb_status;
+    pub fn hb_layer_norm_forward(device: i32, x: *const c_void, dtype: i32, x_stride: u64, n_rows:
+        u64, width: u32, weight: *const c_void, bias: *const c_void, param_type: i32, eps: f32, y:
+        *mut c_void, mean: *mut f32, rstd: *mut f32, stream: *mut c_void) -> hb_status;
+    pub fn hb_layer_norm_backward_workspace(n_rows: u64, width: u32, bytes: *mut u64) -> hb_status;
+    pub fn hb_layer_norm_backward(device: i32, dy: *const c_void, dy_stride: u64, x: *const c_void,
+        x_stride: u64, dtype: i32, n_rows: u64, width: u32, weight: *const c_void, param_type: i32,
+        mean: *const f32, rstd: *const f32, dx: *mut c_void, dweight: *mut c_void, dbias: *mut
+        c_void, workspace: *mut c_void, workspace_bytes: u64, stream: *mut c_void) -> hb_status;
+    pub fn hb_linear_xent_forward_workspace(n_rows: u64, width: u32, n_classes: u64, dtype: i32,
+        bytes: *mut u64) -> hb_status;
+    pub fn hb_linear_xent_forward(device: i32, x: *const c_void, x_stride: u64, w: *const c_void,
+        w_stride: u64, dtype: i32, labels: *const c_void, label_type: i32, n_rows: u64, width: u32,
+        n_classes: u64, loss: *mut f32, lse: *mut f32, workspace: *mut c_void, workspace_bytes: u64,
+        stream: *mut c_void) -> hb_status;
+    pub fn hb_linear_xent_backward_workspace(n_rows: u64, width: u32, n_classes: u64, dtype: i32,
+        bytes: *mut u64) -> hb_status;
+    pub fn hb_linear_xent_backward(device: i32, dloss: *const f32, dloss_stride: u64, x: *const
+        c_void, x_stride: u64, w: *const c_void, w_stride: u64, dtype: i32, labels: *const c_void,
+        label_type: i32, lse: *const f32, n_rows: u64, width: u32, n_classes: u64, dx: *mut c_void,
+        dw: *mut c_void, workspace: *mut c_void, workspace_bytes: u64, stream: *mut c_void) ->
+        hb_status;
+    pub fn hb_grad_norm_workspace(n_tensors: i32, sizes: *const u64, bytes: *mut u64) -> hb_status;
+    pub fn hb_grad_norm(device: i32, n_tensors: i32, tensors: *const *const c_void, sizes: *const
+        u64, dtypes: *const i32, norm: *mut f32, workspace: *mut c_void, workspace_bytes: u64,
+        stream: *mut c_void) -> hb_status;
+    pub fn hb_clip_grad_norm(device: i32, n_tensors: i32, tensors: *const *const c_void, outs:
+        *const *mut c_void, sizes: *const u64, dtypes: *const i32, max_norm: f32, norm: *mut f32,
+        workspace: *mut c_void, workspace_bytes: u64, stream: *mut c_void) -> hb_status;
 }
