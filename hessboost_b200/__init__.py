@@ -295,10 +295,10 @@ SIGNATURES = {
     "hb_layer_norm_backward_workspace": [_u64, _u32, _u64p],
     "hb_layer_norm_backward": [_i32, _vp, _u64, _vp, _u64, _i32, _u64, _u32, _vp, _i32, _vp, _vp, _vp, _vp, _vp,
         _vp, _u64, _vp],
-    "hb_linear_xent_forward_workspace": [_u64, _u32, _u64, _i32, _u64p],
+    "hb_linear_xent_forward_workspace": [_i32, _vp, _u64, _vp, _u64, _i32, _u64, _u32, _u64, _u64p],
     "hb_linear_xent_forward": [_i32, _vp, _u64, _vp, _u64, _i32, _vp, _i32, _u64, _u32, _u64, _vp, _vp, _vp, _u64,
         _vp],
-    "hb_linear_xent_backward_workspace": [_u64, _u32, _u64, _i32, _u64p],
+    "hb_linear_xent_backward_workspace": [_i32, _vp, _u64, _vp, _u64, _i32, _u64, _u32, _u64, _u64p],
     "hb_linear_xent_backward": [_i32, _vp, _u64, _vp, _u64, _vp, _u64, _i32, _vp, _i32, _vp, _u64, _u32, _u64,
         _vp, _vp, _vp, _u64, _vp],
     "hb_grad_norm_workspace": [_i32, _vp, _u64p],

@@ -23,7 +23,10 @@ int sm_count(int device) {
   const bool kept = device >= 0 && device < 64;
   int n = kept ? g_sms[device].load(std::memory_order_relaxed) : 0;
   if (!n) {
-    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device) != cudaSuccess || n < 1) n = 1;
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device) != cudaSuccess || n < 1) {
+      cudaGetLastError();
+      return 1;  // no such device: the call is refused later
+    }
     if (kept) g_sms[device].store(n, std::memory_order_relaxed);
   }
   return n;

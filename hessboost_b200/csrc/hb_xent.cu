@@ -5,40 +5,21 @@
 //
 // A label outside [0, n_classes) is a row without a label: its loss is 0
 // and it takes no part in the gradients. The forward pass keeps only lse;
-// the backward pass computes the logits again, a piece of the classes at a
-// time.
+// the backward pass computes the logits again, a piece of the classes (and a
+// chunk of the rows) at a time, so that what is held of G stays below
+// kGradElements. The products are hb_xent_mma.cu's.
 #include <algorithm>
 #include <cmath>
 
-#include "hb_head.h"
+#include "hb_xent.h"
 
 namespace hb {
 namespace head {
 namespace {
 
-constexpr int kTile = 64;    // rows and classes of a CTA's tile of logits
-constexpr int kStep = 16;    // columns of a step
-constexpr int kSplits = 64;  // parts of the classes in the forward pass
-
-// c[4][4] += A[row0 + 4 ty + i][k] B[col0 + 4 tx + j][k] over k in [0, kn),
-// A and B read through element (row, k) functions that give 0 outside.
-template <typename FA, typename FB>
-__device__ __forceinline__ void tile_product(uint64_t kn, FA a, FB b, float (&c)[4][4], float (*sa)[kTile + 1],
-                                             float (*sb)[kTile + 1]) {
-  const int t = threadIdx.x, tx = t & 15, ty = t >> 4;
-  for (uint64_t k0 = 0; k0 < kn; k0 += kStep) {
-    for (int i = t; i < kTile * kStep; i += 256) {
-      const int r = i / kStep, k = i % kStep;
-      sa[k][r] = k0 + k < kn ? a(r, k0 + k) : 0.0f;
-      sb[k][r] = k0 + k < kn ? b(r, k0 + k) : 0.0f;
-    }
-    __syncthreads();
-    for (int k = 0; k < kStep; ++k)
-      for (int i = 0; i < 4; ++i)
-        for (int j = 0; j < 4; ++j) c[i][j] = fmaf(sa[k][4 * ty + i], sb[k][4 * tx + j], c[i][j]);
-    __syncthreads();
-  }
-}
+constexpr int64_t kGradElements = 40ll << 20;  // of G held at a time (80 MiB in bf16)
+constexpr uint64_t kPartBytes = 64ull << 20;   // of the stats' parts held at a time
+constexpr int kFinishThreads = 256;
 
 template <typename L>
 __device__ __forceinline__ int64_t label_of(const L* labels, uint64_t r, uint64_t n_classes) {
@@ -46,65 +27,37 @@ __device__ __forceinline__ int64_t label_of(const L* labels, uint64_t r, uint64_
   return v >= 0 && v < (int64_t)n_classes ? v : -1;
 }
 
-// Split blockIdx.y of the classes: each row's maximum, sum of exp(z - max)
-// and, where the split holds it, its label's logit.
-template <typename T, typename L>
-__global__ void __launch_bounds__(256)
-    k_xent_parts(const T* __restrict__ x, uint64_t x_stride, const T* __restrict__ w, uint64_t w_stride,
-                 const L* __restrict__ labels, uint64_t n_rows, uint32_t width, uint64_t n_classes,
-                 float2* __restrict__ part, float* __restrict__ at_label) {
-  __shared__ float sa[kStep][kTile + 1], sb[kStep][kTile + 1];
-  __shared__ float2 sp[kTile][16];
-  const uint64_t row0 = (uint64_t)blockIdx.x * kTile;
-  const uint64_t tiles = (n_classes + kTile - 1) / kTile;
-  const uint64_t t0 = tiles * blockIdx.y / gridDim.y, t1 = tiles * (blockIdx.y + 1) / gridDim.y;
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  float m[4], s[4];
-  int64_t label[4];
-  for (int i = 0; i < 4; ++i) {
-    m[i] = -INFINITY, s[i] = 0.0f;
-    const uint64_t r = row0 + 4 * ty + i;
-    label[i] = r < n_rows ? label_of(labels, r, n_classes) : -1;
-  }
-  for (uint64_t tl = t0; tl < t1; ++tl) {
-    const uint64_t col0 = tl * kTile;
-    float c[4][4] = {};
-    tile_product(
-        width, [&](int r, uint64_t k) { return row0 + r < n_rows ? to_f32(x[(row0 + r) * x_stride + k]) : 0.0f; },
-        [&](int r, uint64_t k) { return col0 + r < n_classes ? to_f32(w[(col0 + r) * w_stride + k]) : 0.0f; }, c, sa, sb);
-    for (int i = 0; i < 4; ++i)
-      for (int j = 0; j < 4; ++j) {
-        const uint64_t v = col0 + 4 * tx + j;
-        if (v >= n_classes) continue;
-        const float z = c[i][j];
-        if ((int64_t)v == label[i]) at_label[row0 + 4 * ty + i] = z;
-        const float top = fmaxf(m[i], z);
-        s[i] = (m[i] == top ? s[i] : s[i] * expf(m[i] - top)) + (z == top ? 1.0f : expf(z - top));
-        m[i] = top;
-      }
-  }
-  for (int i = 0; i < 4; ++i) sp[4 * ty + i][tx] = make_float2(m[i], s[i]);
-  __syncthreads();
-  if (threadIdx.x < kTile && row0 + threadIdx.x < n_rows) {
-    float2 a = sp[threadIdx.x][0];
-    for (int j = 1; j < 16; ++j) {
-      const float2 b = sp[threadIdx.x][j];
-      const float top = fmaxf(a.x, b.x);
-      a.y = (a.x == top ? a.y : a.y * expf(a.x - top)) + (b.x == top ? b.y : b.y * expf(b.x - top));
-      a.x = top;
+// x in bf16 pieces, out[plane][row][padded], zero past `width`; where labels
+// are given, rows without one are zero (whatever they hold, a product with
+// their zero row of G is to add nothing).
+template <typename T, typename L, int kPlanes>
+__global__ void k_xent_pack(const T* __restrict__ x, uint64_t x_stride, uint64_t n_rows, uint32_t width,
+                            uint32_t padded, const L* __restrict__ labels, uint64_t n_classes,
+                            __nv_bfloat16* __restrict__ out) {
+  const uint64_t total = n_rows * padded;
+  for (uint64_t i = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (uint64_t)gridDim.x * blockDim.x) {
+    const uint64_t r = i / padded;
+    const uint32_t d = (uint32_t)(i - r * padded);
+    float v = 0.0f;
+    if (d < width && (!labels || label_of(labels, r, n_classes) >= 0)) v = to_f32(x[r * x_stride + d]);
+#pragma unroll
+    for (int q = 0; q < kPlanes; ++q) {
+      const __nv_bfloat16 b = __float2bfloat16_rn(v);
+      out[q * total + i] = b;
+      if (q + 1 < kPlanes) v -= __bfloat162float(b);
     }
-    part[(uint64_t)blockIdx.y * n_rows + row0 + threadIdx.x] = a;
   }
 }
 
+// Joins the tiles' (max, sum) of each row in class order.
 template <typename L>
-__global__ void k_xent_join(const float2* __restrict__ part, int splits, const float* __restrict__ at_label,
+__global__ void k_xent_join(const float2* __restrict__ part, int parts, const float* __restrict__ at_label,
                             const L* __restrict__ labels, uint64_t n_rows, uint64_t n_classes,
                             float* __restrict__ loss, float* __restrict__ lse) {
   const uint64_t r = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x;
   if (r >= n_rows) return;
   float2 a = part[r];
-  for (int i = 1; i < splits; ++i) {
+  for (int i = 1; i < parts; ++i) {
     const float2 b = part[(uint64_t)i * n_rows + r];
     const float top = fmaxf(a.x, b.x);
     a.y = (a.x == top ? a.y : a.y * expf(a.x - top)) + (b.x == top ? b.y : b.y * expf(b.x - top));
@@ -115,103 +68,156 @@ __global__ void k_xent_join(const float2* __restrict__ part, int splits, const f
   loss[r] = label_of(labels, r, n_classes) >= 0 ? l - at_label[r] : 0.0f;
 }
 
-// G of the classes [v0, v0 + vn): g[r][v - v0], f32.
-template <typename T, typename L>
-__global__ void __launch_bounds__(256)
-    k_xent_grad(const T* __restrict__ x, uint64_t x_stride, const T* __restrict__ w, uint64_t w_stride,
-                const L* __restrict__ labels, const float* __restrict__ dloss, uint64_t dloss_stride,
-                const float* __restrict__ lse, uint64_t n_rows, uint32_t width, uint64_t n_classes, uint64_t v0,
-                uint64_t vn, float* __restrict__ g) {
-  __shared__ float sa[kStep][kTile + 1], sb[kStep][kTile + 1];
-  const uint64_t row0 = (uint64_t)blockIdx.x * kTile, col0 = (uint64_t)blockIdx.y * kTile;
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  float c[4][4] = {};
-  tile_product(
-      width, [&](int r, uint64_t k) { return row0 + r < n_rows ? to_f32(x[(row0 + r) * x_stride + k]) : 0.0f; },
-      [&](int r, uint64_t k) { return col0 + r < vn ? to_f32(w[(v0 + col0 + r) * w_stride + k]) : 0.0f; }, c, sa, sb);
-  for (int i = 0; i < 4; ++i) {
-    const uint64_t r = row0 + 4 * ty + i;
-    if (r >= n_rows) continue;
-    const int64_t label = label_of(labels, r, n_classes);
-    const float each = label >= 0 ? dloss[r * dloss_stride] : 0.0f, l = lse[r];
-    for (int j = 0; j < 4; ++j) {
-      const uint64_t v = col0 + 4 * tx + j;
-      if (v < vn) g[r * vn + v] = label < 0 ? 0.0f : each * (expf(c[i][j] - l) - ((int64_t)(v0 + v) == label ? 1.0f : 0.0f));
-    }
+// out[r][d] = the sum of the splits' accumulators, in their order.
+template <typename T>
+__global__ void k_xent_finish(const float* __restrict__ acc, int splits, uint64_t split_rows, uint64_t n_rows,
+                              uint32_t width, uint32_t acc_stride, T* __restrict__ out) {
+  const uint64_t total = n_rows * width;
+  for (uint64_t i = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (uint64_t)gridDim.x * blockDim.x) {
+    const uint64_t r = i / width, at = r * acc_stride + (i - r * width);
+    float v = acc[at];
+    for (int s = 1; s < splits; ++s) v += acc[s * split_rows * acc_stride + at];
+    out[i] = from_f32<T>(v);
   }
 }
 
-// acc[r][d] (+)= sum over v of g[r][v] W[v0 + v][d]
-template <typename T>
-__global__ void __launch_bounds__(256)
-    k_xent_dx(const float* __restrict__ g, const T* __restrict__ w, uint64_t w_stride, uint64_t n_rows,
-              uint32_t width, uint64_t v0, uint64_t vn, float* __restrict__ acc, T* __restrict__ dx, int first, int last) {
-  __shared__ float sa[kStep][kTile + 1], sb[kStep][kTile + 1];
-  const uint64_t row0 = (uint64_t)blockIdx.x * kTile, col0 = (uint64_t)blockIdx.y * kTile;
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  float c[4][4] = {};
-  tile_product(
-      vn, [&](int r, uint64_t k) { return row0 + r < n_rows ? g[(row0 + r) * vn + k] : 0.0f; },
-      [&](int r, uint64_t k) { return col0 + r < width ? to_f32(w[(v0 + k) * w_stride + col0 + r]) : 0.0f; }, c, sa, sb);
-  for (int i = 0; i < 4; ++i)
-    for (int j = 0; j < 4; ++j) {
-      const uint64_t r = row0 + 4 * ty + i, d = col0 + 4 * tx + j;
-      if (r >= n_rows || d >= width) continue;
-      const float v = first ? c[i][j] : acc[r * width + d] + c[i][j];
-      if (last) dx[r * width + d] = from_f32<T>(v);
-      else acc[r * width + d] = v;
-    }
+// ---- plans ---------------------------------------------------------------
+struct Operand {
+  bool packed;
+  uint64_t bytes;  // of its packed form
+};
+struct Sizes {
+  uint64_t n_rows, n_classes;
+  uint32_t width, padded;
+  int planes;
+};
+
+Sizes sizes_of(int32_t dtype, uint64_t n_rows, uint32_t width, uint64_t n_classes) {
+  return {n_rows, n_classes, width, (uint32_t)round_up(width, 8), dtype == HB_F32 ? 3 : 1};
+}
+// TMA takes bf16 rows as they are where the address and the row stride are
+// whole 16-byte units.
+Operand operand_of(const Sizes& z, int32_t dtype, const void* p, uint64_t stride, uint64_t rows, bool always) {
+  const bool packed = always || dtype != HB_BF16 || !aligned(p, 16) || stride % 8;
+  return {packed, packed ? round_up(2ull * z.planes * rows * z.padded, 256) : 0};
 }
 
-// dW[v0 + v][d] = sum over r of g[r][v] x[r][d]
-template <typename T>
-__global__ void __launch_bounds__(256)
-    k_xent_dw(const float* __restrict__ g, const T* __restrict__ x, uint64_t x_stride, uint64_t n_rows,
-              uint32_t width, uint64_t v0, uint64_t vn, T* __restrict__ dw) {
-  __shared__ float sa[kStep][kTile + 1], sb[kStep][kTile + 1];
-  const uint64_t row0 = (uint64_t)blockIdx.x * kTile, col0 = (uint64_t)blockIdx.y * kTile;
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  float c[4][4] = {};
-  tile_product(
-      n_rows, [&](int r, uint64_t k) { return row0 + r < vn ? g[k * vn + row0 + r] : 0.0f; },
-      [&](int r, uint64_t k) { return col0 + r < width ? to_f32(x[k * x_stride + col0 + r]) : 0.0f; }, c, sa, sb);
-  for (int i = 0; i < 4; ++i)
-    for (int j = 0; j < 4; ++j) {
-      const uint64_t v = row0 + 4 * ty + i, d = col0 + 4 * tx + j;
-      if (v < vn && d < width) dw[(v0 + v) * width + d] = from_f32<T>(c[i][j]);
-    }
+// Columns of a tile: 256 where there are enough of them and enough tiles
+// for the SMs, else fewer (in steps of 64).
+int tile_cols(uint64_t cols, uint64_t m_tiles, int sms) {
+  int n = cols >= 256 ? 256 : (int)round_up(cols, 64);
+  while (n > 64 && m_tiles * ((cols + n - 1) / n) < (uint64_t)sms) n = n > 128 ? 128 : 64;
+  return n;
+}
+// Parts of k: enough tiles for the SMs, at least 4 steps of 64 each.
+int k_splits(uint64_t tiles, int k_blocks, int sms) {
+  if (tiles >= (uint64_t)sms) return 1;
+  const int want = (int)((sms + tiles - 1) / tiles);
+  return std::max(1, std::min(want, k_blocks / 4));
 }
 
-// Classes of a piece: G of a piece takes about 64 MiB.
-uint64_t piece_of(uint64_t n_rows, uint64_t n_classes) {
-  const uint64_t most = (16ull << 20) / std::max<uint64_t>(n_rows, 1) / kTile * kTile;
-  return std::min(n_classes, std::min<uint64_t>(65535ull * kTile, std::max<uint64_t>(most, kTile)));
+struct Forward {
+  Operand x, w;
+  int n_size, n_tiles;
+  uint64_t chunk, part, at_label, bytes;
+};
+Forward forward_plan(const Sizes& z, int32_t dtype, const void* x, uint64_t x_stride, const void* w, uint64_t w_stride, int sms) {
+  Forward f;
+  f.x = operand_of(z, dtype, x, x_stride, z.n_rows, false);
+  f.w = operand_of(z, dtype, w, w_stride, z.n_classes, false);
+  f.n_size = tile_cols(z.n_classes, (z.n_rows + 127) / 128, sms);
+  f.n_tiles = (int)((z.n_classes + f.n_size - 1) / f.n_size);
+  f.chunk = std::min<uint64_t>(z.n_rows, std::max<uint64_t>(128, kPartBytes / (8ull * f.n_tiles) / 128 * 128));
+  f.part = round_up(8ull * f.n_tiles * f.chunk, 256);
+  f.at_label = round_up(4 * f.chunk, 256);
+  f.bytes = f.x.bytes + f.w.bytes + f.part + f.at_label;
+  return f;
 }
 
-hb_status check_xent(const void* x, uint64_t x_stride, const void* w, uint64_t w_stride, int32_t dtype, const void* labels,
-                     int32_t label_type, uint64_t n_rows, uint32_t width, uint64_t n_classes) {
-  HB_HEAD_REQUIRE(dtype == HB_F32 || dtype == HB_BF16, "x and w are f32 or bf16");
-  HB_HEAD_REQUIRE(label_type == HB_I32 || label_type == HB_I64, "unknown label type");
-  HB_HEAD_REQUIRE(width >= 1 && width <= (1u << 20), "width must be in [1, 2^20]");
-  HB_HEAD_REQUIRE(n_classes >= 1 && n_classes < (1ull << 31), "n_classes must be in [1, 2^31)");
-  HB_HEAD_REQUIRE(n_rows < (1ull << 31), "at most 2^31 - 1 rows");
-  HB_HEAD_REQUIRE(w && (!n_rows || (x && labels)), "x, w or labels is NULL");
-  HB_HEAD_REQUIRE(x_stride >= width || n_rows <= 1, "x_stride is below width");
-  HB_HEAD_REQUIRE(w_stride >= width || n_classes <= 1, "w_stride is below width");
-  HB_HEAD_REQUIRE(aligned(x, size_of(dtype)) && aligned(w, size_of(dtype)) && aligned(labels, label_type == HB_I32 ? 4 : 8),
-                  "a buffer is not aligned to its type");
-  return HB_OK;
-}
-
-uint64_t forward_bytes(uint64_t n_rows) { return round_up(4 * n_rows, 256) + 8 * kSplits * n_rows; }
-uint64_t backward_bytes(uint64_t n_rows, uint32_t width, uint64_t n_classes) {
-  return round_up(4 * n_rows * piece_of(n_rows, n_classes), 256) + 4 * n_rows * width;
+struct Backward {
+  Operand x, w;
+  uint64_t piece, chunk, pieces, chunks;
+  uint64_t g_stride;                      // elements of a row of G
+  int grad_n, out_n;                      // tile columns of grad, and of dx and dw
+  int dx_splits, dw_splits;
+  bool dx_acc, dw_acc;
+  uint32_t acc_stride;
+  uint64_t dw_rows;                       // rows of a dw accumulator
+  uint64_t g_bytes, dx_bytes, dw_bytes, bytes;
+};
+Backward backward_plan(const Sizes& z, int32_t dtype, const void* x, uint64_t x_stride, const void* w, uint64_t w_stride, int sms) {
+  Backward b;
+  b.x = operand_of(z, dtype, x, x_stride, z.n_rows, true);
+  b.w = operand_of(z, dtype, w, w_stride, z.n_classes, false);
+  const uint64_t most = (uint64_t)kGradElements / z.planes;
+  const uint64_t least = 4096;  // classes of a piece, where there are as many
+  b.chunk = std::min(z.n_rows, std::max<uint64_t>(most / std::min(z.n_classes, least) / 128 * 128, 128));
+  b.chunks = (z.n_rows + b.chunk - 1) / b.chunk;
+  b.piece = std::min(z.n_classes, std::max<uint64_t>(most / b.chunk / 256 * 256, 256));
+  b.pieces = (z.n_classes + b.piece - 1) / b.piece;
+  b.piece = std::min(b.piece, round_up((z.n_classes + b.pieces - 1) / b.pieces, 256));
+  b.g_stride = round_up(b.piece, 64);
+  const uint64_t row_tiles = (b.chunk + 127) / 128, class_tiles = (b.piece + 127) / 128;
+  b.grad_n = tile_cols(b.piece, row_tiles, sms);
+  b.out_n = tile_cols(z.width, row_tiles + class_tiles, sms);
+  const uint64_t out_tiles = (z.width + b.out_n - 1) / b.out_n;
+  b.dx_splits = k_splits(row_tiles * out_tiles, (int)((b.piece + 63) / 64), sms);
+  b.dw_splits = k_splits(class_tiles * out_tiles, (int)((b.chunk + 63) / 64), sms);
+  b.dx_acc = b.dx_splits > 1 || b.pieces > 1;
+  b.dw_acc = b.dw_splits > 1 || b.chunks > 1;
+  b.acc_stride = (uint32_t)round_up(z.width, 4);
+  b.dw_rows = b.chunks > 1 ? z.n_classes : b.piece;
+  b.g_bytes = round_up(2ull * z.planes * b.chunk * b.g_stride, 256);
+  b.dx_bytes = b.dx_acc ? round_up(4ull * b.dx_splits * b.chunk * b.acc_stride, 256) : 0;
+  b.dw_bytes = b.dw_acc ? round_up(4ull * b.dw_splits * b.dw_rows * b.acc_stride, 256) : 0;
+  b.bytes = b.x.bytes + b.w.bytes + b.g_bytes + b.dx_bytes + b.dw_bytes;
+  return b;
 }
 
 template <typename F>
 void with_xent_types(int32_t dtype, int32_t label_type, F&& f) {
   auto g = [&](auto t) { if (label_type == HB_I32) f(t, int32_t{}); else f(t, int64_t{}); };
   if (dtype == HB_F32) g(float{}); else g(__nv_bfloat16{});
+}
+
+int grid_for(uint64_t threads, int block, int sms) {
+  return (int)std::max<uint64_t>(1, std::min<uint64_t>((threads + block - 1) / block, (uint64_t)sms * 16));
+}
+
+// The operand's map with boxes of 64 rows, after packing it to `at` where
+// that is needed.
+bool operand(CUtensorMap* map, const Operand& o, const Sizes& z, int32_t dtype, const void* p, uint64_t stride, uint64_t rows,
+             const void* labels, int32_t label_type, void* at, int sms, cudaStream_t s) {
+  if (!o.packed) return mma_map(map, p, z.width, rows, 1, stride, stride * rows, 64);
+  const uint64_t total = rows * z.padded;
+  with_xent_types(dtype, label_type, [&](auto t, auto l) {
+    using T = decltype(t);
+    using L = decltype(l);
+    constexpr int kPlanes = sizeof(T) == 4 ? 3 : 1;
+    k_xent_pack<T, L, kPlanes><<<grid_for(total, 256, sms), 256, 0, s>>>((const T*)p, stride, rows, z.width, z.padded,
+                                                                   (const L*)labels, z.n_classes, (__nv_bfloat16*)at);
+  });
+  return mma_map(map, at, z.padded, rows, z.planes, z.padded, total, 64);
+}
+
+hb_status check_xent(const void* x, uint64_t x_stride, const void* w, uint64_t w_stride, int32_t dtype, uint64_t n_rows,
+                     uint32_t width, uint64_t n_classes) {
+  HB_HEAD_REQUIRE(dtype == HB_F32 || dtype == HB_BF16, "x and w are f32 or bf16");
+  HB_HEAD_REQUIRE(width >= 1 && width <= (1u << 20), "width must be in [1, 2^20]");
+  HB_HEAD_REQUIRE(n_classes >= 1 && n_classes < (1ull << 31) - 512, "n_classes must be in [1, 2^31 - 512)");
+  HB_HEAD_REQUIRE(n_rows < (1ull << 31) - 512, "at most 2^31 - 513 rows");
+  HB_HEAD_REQUIRE(w && (!n_rows || x), "x or w is NULL");
+  HB_HEAD_REQUIRE(x_stride >= width || n_rows <= 1, "x_stride is below width");
+  HB_HEAD_REQUIRE(w_stride >= width || n_classes <= 1, "w_stride is below width");
+  HB_HEAD_REQUIRE(x_stride < (1ull << 38) && w_stride < (1ull << 38), "a stride is too large");
+  HB_HEAD_REQUIRE(aligned(x, size_of(dtype)) && aligned(w, size_of(dtype)), "a buffer is not aligned to its type");
+  return HB_OK;
+}
+hb_status check_labels(const void* labels, int32_t label_type, uint64_t n_rows) {
+  HB_HEAD_REQUIRE(label_type == HB_I32 || label_type == HB_I64, "unknown label type");
+  HB_HEAD_REQUIRE(labels || !n_rows, "labels is NULL");
+  HB_HEAD_REQUIRE(aligned(labels, label_type == HB_I32 ? 4 : 8), "labels is not aligned to its type");
+  return HB_OK;
 }
 
 }  // namespace
@@ -222,10 +228,13 @@ using namespace hb::head;
 
 extern "C" {
 
-hb_status hb_linear_xent_forward_workspace(uint64_t n_rows, uint32_t width, uint64_t n_classes, int32_t dtype, uint64_t* bytes) {
+hb_status hb_linear_xent_forward_workspace(int32_t device, const void* x, uint64_t x_stride, const void* w, uint64_t w_stride,
+                                           int32_t dtype, uint64_t n_rows, uint32_t width, uint64_t n_classes,
+                                           uint64_t* bytes) {
   begin_call();
-  HB_HEAD_REQUIRE(bytes && n_rows < (1ull << 31), "bytes is NULL or too many rows");
-  *bytes = forward_bytes(n_rows);
+  if (hb_status st = check_xent(x, x_stride, w, w_stride, dtype, n_rows, width, n_classes)) return st;
+  HB_HEAD_REQUIRE(bytes, "bytes is NULL");
+  *bytes = n_rows ? forward_plan(sizes_of(dtype, n_rows, width, n_classes), dtype, x, x_stride, w, w_stride, sm_count(device)).bytes : 0;
   return HB_OK;
 }
 
@@ -234,31 +243,58 @@ hb_status hb_linear_xent_forward(int32_t device, const void* x, uint64_t x_strid
                                  uint32_t width, uint64_t n_classes, float* loss, float* lse, void* workspace,
                                  uint64_t workspace_bytes, void* stream) {
   begin_call();
-  if (hb_status st = check_xent(x, x_stride, w, w_stride, dtype, labels, label_type, n_rows, width, n_classes)) return st;
+  if (hb_status st = check_xent(x, x_stride, w, w_stride, dtype, n_rows, width, n_classes)) return st;
+  if (hb_status st = check_labels(labels, label_type, n_rows)) return st;
   if (!n_rows) return HB_OK;
   HB_HEAD_REQUIRE(loss && lse && aligned(loss, 4) && aligned(lse, 4), "loss or lse is NULL or not aligned");
-  HB_HEAD_REQUIRE(workspace && aligned(workspace, 256) && workspace_bytes >= forward_bytes(n_rows),
+  const Sizes z = sizes_of(dtype, n_rows, width, n_classes);
+  const int sms = sm_count(device);
+  const Forward f = forward_plan(z, dtype, x, x_stride, w, w_stride, sms);
+  HB_HEAD_REQUIRE(workspace && aligned(workspace, 256) && workspace_bytes >= f.bytes,
                   "workspace is too small or not 256-byte aligned");
   DeviceScope dev(device);
   if (!dev.ok()) return fail(HB_REFUSED, "no such device");
   cudaStream_t s = (cudaStream_t)stream;
-  float* at_label = (float*)workspace;
-  float2* part = (float2*)((char*)workspace + round_up(4 * n_rows, 256));
-  const int splits = (int)std::min<uint64_t>(kSplits, (n_classes + kTile - 1) / kTile);
-  with_xent_types(dtype, label_type, [&](auto t, auto l) {
-    using T = decltype(t);
-    using L = decltype(l);
-    k_xent_parts<T, L><<<dim3((unsigned)((n_rows + kTile - 1) / kTile), splits), 256, 0, s>>>(
-        (const T*)x, x_stride, (const T*)w, w_stride, (const L*)labels, n_rows, width, n_classes, part, at_label);
-    k_xent_join<L><<<(int)((n_rows + 255) / 256), 256, 0, s>>>(part, splits, at_label, (const L*)labels, n_rows, n_classes, loss, lse);
-  });
+  char* at = (char*)workspace;
+  MmaParams p{};
+  if (!operand(&p.x, f.x, z, dtype, x, x_stride, n_rows, nullptr, label_type, at, sms, s) ||
+      !operand(&p.w, f.w, z, dtype, w, w_stride, n_classes, nullptr, label_type, at + f.x.bytes, sms, s))
+    return fail(HB_DEVICE_FAILED, "tensor map");
+  at += f.x.bytes + f.w.bytes;
+  p.part = (float2*)at;
+  p.at_label = (float*)(at + f.part);
+  p.pairs = z.planes == 3 ? 6 : 1;
+  p.planes = z.planes;
+  p.n_classes = (int)n_classes;
+  p.all_classes = (int64_t)n_classes;
+  p.width = (int)width;
+  p.label_type = label_type;
+  p.n_jobs = 1;
+  const uint64_t label_size = label_type == HB_I32 ? 4 : 8;
+  for (uint64_t r0 = 0; r0 < n_rows; r0 += f.chunk) {
+    const uint64_t rows = std::min(f.chunk, n_rows - r0);
+    p.n_rows = (int)rows;
+    p.row0 = (int)r0;
+    p.labels = (const char*)labels + r0 * label_size;
+    p.part_stride = rows;
+    p.jobs[0] = MmaJob{kJobStats, 0, (int)((rows + 127) / 128), f.n_tiles, f.n_size, (int)((width + 63) / 64), 1, 1, {}};
+    if (hb_status st = mma_launch(p, sms, s)) return st;
+    with_xent_types(dtype, label_type, [&](auto, auto l) {
+      using L = decltype(l);
+      k_xent_join<L><<<(int)((rows + 255) / 256), 256, 0, s>>>(p.part, f.n_tiles, p.at_label, (const L*)p.labels, rows, n_classes,
+                                                           loss + r0, lse + r0);
+    });
+  }
   return launched("hb_linear_xent_forward");
 }
 
-hb_status hb_linear_xent_backward_workspace(uint64_t n_rows, uint32_t width, uint64_t n_classes, int32_t dtype, uint64_t* bytes) {
+hb_status hb_linear_xent_backward_workspace(int32_t device, const void* x, uint64_t x_stride, const void* w, uint64_t w_stride,
+                                            int32_t dtype, uint64_t n_rows, uint32_t width, uint64_t n_classes,
+                                            uint64_t* bytes) {
   begin_call();
-  HB_HEAD_REQUIRE(bytes && n_rows < (1ull << 31) && n_classes < (1ull << 31) && width <= (1u << 20), "bytes is NULL or sizes out of range");
-  *bytes = backward_bytes(n_rows, width, n_classes);
+  if (hb_status st = check_xent(x, x_stride, w, w_stride, dtype, n_rows, width, n_classes)) return st;
+  HB_HEAD_REQUIRE(bytes, "bytes is NULL");
+  *bytes = n_rows ? backward_plan(sizes_of(dtype, n_rows, width, n_classes), dtype, x, x_stride, w, w_stride, sm_count(device)).bytes : 0;
   return HB_OK;
 }
 
@@ -268,36 +304,88 @@ hb_status hb_linear_xent_backward(int32_t device, const float* dloss, uint64_t d
                                   uint32_t width, uint64_t n_classes, void* dx, void* dw, void* workspace,
                                   uint64_t workspace_bytes, void* stream) {
   begin_call();
-  if (hb_status st = check_xent(x, x_stride, w, w_stride, dtype, labels, label_type, n_rows, width, n_classes)) return st;
+  if (hb_status st = check_xent(x, x_stride, w, w_stride, dtype, n_rows, width, n_classes)) return st;
+  if (hb_status st = check_labels(labels, label_type, n_rows)) return st;
   HB_HEAD_REQUIRE(dw && (!n_rows || (dloss && lse && dx)), "dloss, lse, dx or dw is NULL");
   HB_HEAD_REQUIRE(aligned(dloss, 4) && aligned(lse, 4) && aligned(dx, size_of(dtype)) && aligned(dw, size_of(dtype)),
                   "a buffer is not aligned to its type");
-  HB_HEAD_REQUIRE(!n_rows || (workspace && aligned(workspace, 256) && workspace_bytes >= backward_bytes(n_rows, width, n_classes)),
-                  "workspace is too small or not 256-byte aligned");
+  const Sizes z = sizes_of(dtype, n_rows, width, n_classes);
+  const int sms = sm_count(device);
+  Backward b{};
+  if (n_rows) {
+    b = backward_plan(z, dtype, x, x_stride, w, w_stride, sms);
+    HB_HEAD_REQUIRE(workspace && aligned(workspace, 256) && workspace_bytes >= b.bytes,
+                    "workspace is too small or not 256-byte aligned");
+  }
   DeviceScope dev(device);
   if (!dev.ok()) return fail(HB_REFUSED, "no such device");
   cudaStream_t s = (cudaStream_t)stream;
   if (!n_rows) {
-    cudaMemsetAsync(dw, 0, n_classes * width * size_of(dtype), s);
-    return launched("hb_linear_xent_backward");
+    if (cudaMemsetAsync(dw, 0, n_classes * width * size_of(dtype), s) != cudaSuccess) return launched("hb_linear_xent_backward");
+    return HB_OK;
   }
-  const uint64_t piece = piece_of(n_rows, n_classes);
-  float* g = (float*)workspace;
-  float* acc = (float*)((char*)workspace + round_up(4 * n_rows * piece, 256));
-  const unsigned row_tiles = (unsigned)((n_rows + kTile - 1) / kTile), d_tiles = (width + kTile - 1) / kTile;
-  with_xent_types(dtype, label_type, [&](auto t, auto l) {
-    using T = decltype(t);
-    using L = decltype(l);
-    for (uint64_t v0 = 0; v0 < n_classes; v0 += piece) {
-      const uint64_t vn = std::min(piece, n_classes - v0);
-      const unsigned v_tiles = (unsigned)((vn + kTile - 1) / kTile);
-      k_xent_grad<T, L><<<dim3(row_tiles, v_tiles), 256, 0, s>>>((const T*)x, x_stride, (const T*)w, w_stride, (const L*)labels,
-                                                             dloss, dloss_stride, lse, n_rows, width, n_classes, v0, vn, g);
-      k_xent_dx<T><<<dim3(row_tiles, d_tiles), 256, 0, s>>>(g, (const T*)w, w_stride, n_rows, width, v0, vn, acc, (T*)dx,
-                                                        v0 == 0, v0 + vn == n_classes);
-      k_xent_dw<T><<<dim3(v_tiles, d_tiles), 256, 0, s>>>(g, (const T*)x, x_stride, n_rows, width, v0, vn, (T*)dw);
+  char* at = (char*)workspace;
+  MmaParams p{};
+  if (!operand(&p.x, b.x, z, dtype, x, x_stride, n_rows, labels, label_type, at, sms, s) ||
+      !operand(&p.w, b.w, z, dtype, w, w_stride, n_classes, nullptr, label_type, at + b.x.bytes, sms, s))
+    return fail(HB_DEVICE_FAILED, "tensor map");
+  at += b.x.bytes + b.w.bytes;
+  void* g = at;
+  float* dx_acc = (float*)(at + b.g_bytes);
+  float* dw_acc = (float*)(at + b.g_bytes + b.dx_bytes);
+  p.pairs = z.planes == 3 ? 6 : 1;
+  p.planes = z.planes;
+  p.all_classes = (int64_t)n_classes;
+  p.width = (int)width;
+  p.label_type = label_type;
+  p.dloss_stride = dloss_stride;
+  p.first_dloss = dloss;
+  const uint64_t label_size = label_type == HB_I32 ? 4 : 8, e = size_of(dtype);
+  const int out_type = dtype == HB_F32 ? kOutF32 : kOutBf16;
+  const int out_tiles = (int)((width + b.out_n - 1) / b.out_n);
+  const auto vec = [&](const void* q) { return (int)(aligned(q, 16) && width * e % 16 == 0); };
+  // dx or dw of `rows` rows from `splits` accumulators
+  const auto finish = [&](const float* acc, int splits, uint64_t split_rows, uint64_t rows, void* to) {
+    const int grid = grid_for(rows * width, kFinishThreads, sms);
+    if (dtype == HB_F32)
+      k_xent_finish<float><<<grid, kFinishThreads, 0, s>>>(acc, splits, split_rows, rows, width, b.acc_stride, (float*)to);
+    else
+      k_xent_finish<__nv_bfloat16><<<grid, kFinishThreads, 0, s>>>(acc, splits, split_rows, rows, width, b.acc_stride, (__nv_bfloat16*)to);
+  };
+  for (uint64_t c = 0; c < b.chunks; ++c) {
+    const uint64_t r0 = c * b.chunk, rows = std::min(b.chunk, n_rows - r0);
+    void* dx_to = (char*)dx + r0 * width * e;
+    p.n_rows = (int)rows;
+    p.row0 = (int)r0;
+    p.labels = (const char*)labels + r0 * label_size;
+    p.dloss = dloss + r0 * dloss_stride;
+    p.lse = lse + r0;
+    for (uint64_t q = 0; q < b.pieces; ++q) {
+      const uint64_t v0 = q * b.piece, classes = std::min(b.piece, n_classes - v0);
+      void* dw_to = (char*)dw + v0 * width * e;
+      p.n_classes = (int)classes;
+      p.class0 = (int)v0;
+      if (!mma_map(&p.g, g, classes, rows, z.planes, b.g_stride, b.chunk * b.g_stride, 64) ||
+          !mma_map(&p.g_out, g, classes, rows, z.planes, b.g_stride, b.chunk * b.g_stride, 32))
+        return fail(HB_DEVICE_FAILED, "tensor map");
+      const int row_tiles = (int)((rows + 127) / 128), class_tiles = (int)((classes + 127) / 128);
+      p.n_jobs = 1;
+      p.jobs[0] = MmaJob{kJobGrad, 0, row_tiles, (int)((classes + b.grad_n - 1) / b.grad_n), b.grad_n, (int)((width + 63) / 64), 1, 1, {}};
+      if (hb_status st = mma_launch(p, sms, s)) return st;
+      const int class_blocks = (int)((classes + 63) / 64), row_blocks = (int)((rows + 63) / 64);
+      MmaOut to_dx{b.dx_acc ? kOutAcc : out_type, q > 0, vec(dx_to), (int)b.chunk, (int)b.acc_stride, dx_acc, dx_to};
+      float* acc = b.chunks > 1 ? dw_acc + v0 * b.acc_stride : dw_acc;
+      MmaOut to_dw{b.dw_acc ? kOutAcc : out_type, c > 0, vec(dw_to), (int)b.dw_rows, (int)b.acc_stride, acc, dw_to};
+      // a last piece or chunk may have fewer steps than splits: the splits
+      // past them add nothing, and are not read
+      p.n_jobs = 2;
+      p.jobs[0] = MmaJob{kJobDw, 0, class_tiles, out_tiles, b.out_n, row_blocks, b.dw_splits, 0, to_dw};
+      p.jobs[1] = MmaJob{kJobDx, 0, row_tiles, out_tiles, b.out_n, class_blocks, b.dx_splits, 0, to_dx};
+      if (hb_status st = mma_launch(p, sms, s)) return st;
+      if (b.dw_acc && c + 1 == b.chunks) finish(acc, b.dw_splits, b.dw_rows, classes, dw_to);
     }
-  });
+    if (b.dx_acc) finish(dx_acc, b.dx_splits, b.chunk, rows, dx_to);
+  }
   return launched("hb_linear_xent_backward");
 }
 

@@ -1,0 +1,66 @@
+// The linear softmax cross entropy's tensor-core products (hb_xent_mma.cu)
+// as its entry points (hb_xent.cu) launch them.
+#pragma once
+
+#include <cuda.h>
+
+#include "hb_head.h"
+
+namespace hb {
+namespace head {
+
+enum MmaKind { kJobStats = 0, kJobGrad = 1, kJobDx = 2, kJobDw = 3 };
+enum MmaOutType { kOutAcc = 0, kOutF32 = 1, kOutBf16 = 2 };
+
+// Where a dx or dw tile goes: f32 accumulators [splits][split_rows]
+// [acc_stride] (added to what an earlier launch left, or set), or the result
+// itself, rows of the layer's width (vec: 16-byte stores will do).
+struct MmaOut {
+  int type, add, vec;
+  int split_rows, acc_stride;
+  float* acc;
+  void* to;
+};
+
+// m_tiles x n_tiles tiles of 128 x n_size, k in steps of 64 shared among
+// `splits` tiles each; m_fast: consecutive tiles go down the rows.
+struct MmaJob {
+  int kind, tiles, m_tiles, n_tiles, n_size, k_blocks, splits, m_fast;
+  MmaOut out;
+};
+
+struct MmaParams {
+  CUtensorMap x, w, g, g_out;  // bf16 [planes][rows][columns]
+  MmaJob jobs[3];
+  int n_jobs, tiles;
+  int pairs, planes;           // 1, 1: bf16; 6, 3: f32 in three pieces
+  int n_rows, n_classes, width;  // of this launch: the chunk's rows, the piece's classes
+  int row0, class0;            // the chunk's first row in x, the piece's first class in w
+  // of the chunk's rows
+  const void* labels;
+  int label_type;
+  int64_t all_classes;
+  const float* first_dloss;    // of the call's first row
+  const float* dloss;
+  uint64_t dloss_stride;
+  const float* lse;
+  float2* part;                // stats: [n_tiles][part_stride]
+  uint64_t part_stride;
+  float* at_label;
+
+  // The row's label, -1 where it has none.
+  __device__ __forceinline__ int64_t label(int row) const {
+    const int64_t v = label_type == HB_I32 ? (int64_t)((const int32_t*)labels)[row] : ((const int64_t*)labels)[row];
+    return v >= 0 && v < all_classes ? v : -1;
+  }
+};
+
+// A map of bf16 [planes][rows][cols] with boxes of 64 columns; strides in
+// elements, multiples of 8, the address 16-byte aligned.
+bool mma_map(CUtensorMap* map, const void* p, uint64_t cols, uint64_t rows, uint64_t planes, uint64_t row_stride,
+             uint64_t plane_stride, int box_rows);
+// Runs the jobs; fills in the tile counts.
+hb_status mma_launch(MmaParams& p, int sms, cudaStream_t s);
+
+}  // namespace head
+}  // namespace hb

@@ -248,9 +248,10 @@ def linear_xent_forward(x, weight, labels):
     L = lib()
     loss = torch.empty(n, dtype=torch.float32, device=x.device)
     lse = torch.empty_like(loss)
-    ws, size = _workspace(L.hb_linear_xent_forward_workspace, x.device, n, width, v, dt)
-    _check(L.hb_linear_xent_forward(dev, x.data_ptr(), max(x.stride(0), width), weight.data_ptr(),
-                                    max(weight.stride(0), width), dt, labels.data_ptr(), _INTS[labels.dtype], n, width,
+    xs, wst = max(x.stride(0), width), max(weight.stride(0), width)
+    ws, size = _workspace(L.hb_linear_xent_forward_workspace, x.device, dev, x.data_ptr(), xs, weight.data_ptr(), wst, dt,
+                          n, width, v)
+    _check(L.hb_linear_xent_forward(dev, x.data_ptr(), xs, weight.data_ptr(), wst, dt, labels.data_ptr(), _INTS[labels.dtype], n, width,
                                     v, loss.data_ptr(), lse.data_ptr(), ws.data_ptr(), size, _stream(dev)),
            "hb_linear_xent_forward")
     return loss, lse
@@ -267,9 +268,11 @@ def linear_xent_backward(dloss, x, weight, labels, lse):
     _device(x, dloss, lse)
     L = lib()
     dx, dw = x.new_empty((n, width)), x.new_empty((v, width))
-    ws, size = _workspace(L.hb_linear_xent_backward_workspace, x.device, n, width, v, dt)
-    _check(L.hb_linear_xent_backward(dev, dloss.data_ptr(), dloss.stride(0), x.data_ptr(), max(x.stride(0), width),
-                                     weight.data_ptr(), max(weight.stride(0), width), dt, labels.data_ptr(),
+    xs, wst = max(x.stride(0), width), max(weight.stride(0), width)
+    ws, size = _workspace(L.hb_linear_xent_backward_workspace, x.device, dev, x.data_ptr(), xs, weight.data_ptr(), wst, dt,
+                          n, width, v)
+    _check(L.hb_linear_xent_backward(dev, dloss.data_ptr(), dloss.stride(0), x.data_ptr(), xs,
+                                     weight.data_ptr(), wst, dt, labels.data_ptr(),
                                      _INTS[labels.dtype], lse.data_ptr(), n, width, v, dx.data_ptr(), dw.data_ptr(),
                                      ws.data_ptr(), size, _stream(dev)), "hb_linear_xent_backward")
     return dx, dw

@@ -494,9 +494,13 @@ hb_status hb_layer_norm_backward(int32_t device, const void* dy, uint64_t dy_str
 /* loss[n] = lse[n] - z[n][label], lse[n] = log(sum over the classes of
  * exp(z[n])), z = x w^T: x n_rows x width, w n_classes x width, both f32 or
  * both bf16. The logits are never kept. A label outside [0, n_classes) is a
- * row without a label: its loss is 0 (its lse is still written). */
-hb_status hb_linear_xent_forward_workspace(uint64_t n_rows, uint32_t width, uint64_t n_classes,
-                                           int32_t dtype, uint64_t* bytes);
+ * row without a label: its loss is 0 (its lse is still written). bf16 rows
+ * that start on 16-byte boundaries (address and stride) are read as they
+ * lie, others are laid out in the workspace first: its size goes by x and w
+ * too. */
+hb_status hb_linear_xent_forward_workspace(int32_t device, const void* x, uint64_t x_stride, const void* w,
+                                          uint64_t w_stride, int32_t dtype, uint64_t n_rows, uint32_t width,
+                                          uint64_t n_classes, uint64_t* bytes);
 hb_status hb_linear_xent_forward(int32_t device, const void* x, uint64_t x_stride, const void* w,
                                  uint64_t w_stride, int32_t dtype, const void* labels, int32_t label_type,
                                  uint64_t n_rows, uint32_t width, uint64_t n_classes, float* loss,
@@ -505,8 +509,9 @@ hb_status hb_linear_xent_forward(int32_t device, const void* x, uint64_t x_strid
  * (dloss_stride 0: one factor for every row); lse from the forward pass. The
  * logits are computed again, a piece of the classes at a time. Rows without
  * a label get 0 and add nothing. */
-hb_status hb_linear_xent_backward_workspace(uint64_t n_rows, uint32_t width, uint64_t n_classes,
-                                            int32_t dtype, uint64_t* bytes);
+hb_status hb_linear_xent_backward_workspace(int32_t device, const void* x, uint64_t x_stride, const void* w,
+                                          uint64_t w_stride, int32_t dtype, uint64_t n_rows, uint32_t width,
+                                          uint64_t n_classes, uint64_t* bytes);
 hb_status hb_linear_xent_backward(int32_t device, const float* dloss, uint64_t dloss_stride, const void* x,
                                   uint64_t x_stride, const void* w, uint64_t w_stride, int32_t dtype,
                                   const void* labels, int32_t label_type, const float* lse,

@@ -178,14 +178,14 @@ extern "C" {
         x_stride: u64, dtype: i32, n_rows: u64, width: u32, weight: *const c_void, param_type: i32,
         mean: *const f32, rstd: *const f32, dx: *mut c_void, dweight: *mut c_void, dbias: *mut
         c_void, workspace: *mut c_void, workspace_bytes: u64, stream: *mut c_void) -> hb_status;
-    pub fn hb_linear_xent_forward_workspace(n_rows: u64, width: u32, n_classes: u64, dtype: i32,
-        bytes: *mut u64) -> hb_status;
+    pub fn hb_linear_xent_forward_workspace(device: i32, x: *const c_void, x_stride: u64, w: *const c_void,
+        w_stride: u64, dtype: i32, n_rows: u64, width: u32, n_classes: u64, bytes: *mut u64) -> hb_status;
     pub fn hb_linear_xent_forward(device: i32, x: *const c_void, x_stride: u64, w: *const c_void,
         w_stride: u64, dtype: i32, labels: *const c_void, label_type: i32, n_rows: u64, width: u32,
         n_classes: u64, loss: *mut f32, lse: *mut f32, workspace: *mut c_void, workspace_bytes: u64,
         stream: *mut c_void) -> hb_status;
-    pub fn hb_linear_xent_backward_workspace(n_rows: u64, width: u32, n_classes: u64, dtype: i32,
-        bytes: *mut u64) -> hb_status;
+    pub fn hb_linear_xent_backward_workspace(device: i32, x: *const c_void, x_stride: u64, w: *const c_void,
+        w_stride: u64, dtype: i32, n_rows: u64, width: u32, n_classes: u64, bytes: *mut u64) -> hb_status;
     pub fn hb_linear_xent_backward(device: i32, dloss: *const f32, dloss_stride: u64, x: *const
         c_void, x_stride: u64, w: *const c_void, w_stride: u64, dtype: i32, labels: *const c_void,
         label_type: i32, lse: *const f32, n_rows: u64, width: u32, n_classes: u64, dx: *mut c_void,

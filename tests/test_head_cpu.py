@@ -65,8 +65,8 @@ def test_xent_refusals():
     for at, v, what in ((7, 1, "f32 or bf16"), (1, None, "NULL"), (10, None, "NULL"), (14, None, "NULL"), (15, None, "NULL"),
                         (1, P + 2, "aligned"), (16, None, "workspace"), (17, 1, "workspace")):
         refused("hb_linear_xent_backward", put(ok, at, v), what)
-    refused("hb_linear_xent_forward_workspace", [1, 1, 1, 0, None], "bytes")
-    refused("hb_linear_xent_backward_workspace", [2**31, 1, 1, 0, ctypes.c_uint64()], "range")
+    refused("hb_linear_xent_forward_workspace", [0, P, 8, P, 8, 0, 1, 8, 1, None], "bytes")
+    refused("hb_linear_xent_backward_workspace", [0, P, 8, P, 8, 0, 2**31, 8, 1, ctypes.c_uint64()], "rows")
 
 
 def test_clip_refusals():
