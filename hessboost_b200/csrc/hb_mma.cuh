@@ -37,14 +37,40 @@ __device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
   return ok != 0;
 }
 
+__device__ __forceinline__ bool bar_try_cluster(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n.reg .pred p;\n"
+      "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n"
+      "selp.u32 %0, 1, 0, p;\n}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+// The address of this CTA's `p` in CTA `rank` of the cluster.
+__device__ __forceinline__ uint32_t peer_addr(uint32_t p, uint32_t rank) {
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(p), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ void bar_arrive_at(uint32_t peer_bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(peer_bar) : "memory");
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
 // A bounded wait: gives up after kWaitTries tries (each may sleep a while in
 // hardware; together well over a second) or once another thread of the CTA
 // has given up, and marks the CTA so. False: gave up.
 constexpr uint32_t kWaitTries = 1u << 24;
+template <bool kCluster = false>
 __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile uint32_t* gave_up) {
-  if (bar_try(bar, parity)) return true;
+  const auto tried = [&] { return kCluster ? bar_try_cluster(bar, parity) : bar_try(bar, parity); };
+  if (tried()) return true;
   for (uint32_t i = 0; i < kWaitTries; ++i) {
-    if (bar_try(bar, parity)) return true;
+    if (tried()) return true;
     if ((i & 63u) == 63u && *gave_up) return false;
   }
   *gave_up = 1u;
@@ -52,11 +78,20 @@ __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile
 }
 
 // ---- TMA -----------------------------------------------------------------
+// kPair: `bar` may be the pair's other CTA's.
+template <bool kPair>
 __device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y, int z) {
-  asm volatile(
-      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst),
-      "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z)
-      : "memory");
+  if constexpr (kPair)
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%3, %4, %5}], "
+        "[%2];" ::"r"(dst),
+        "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z)
+        : "memory");
+  else
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst),
+        "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z)
+        : "memory");
 }
 __device__ __forceinline__ void tma_store(const CUtensorMap* map, uint32_t src, int x, int y, int z) {
   asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(map), "r"(src), "r"(x),
@@ -73,26 +108,54 @@ __device__ __forceinline__ void tma_prefetch(const CUtensorMap* map) {
 }
 
 // ---- tcgen05 ---------------------------------------------------------------
+// kPair: the instruction's form for two CTAs of a cluster that share a tile;
+// tmem_alloc and tmem_free are then called by both, mma_f16 and mma_commit by
+// the first.
+template <bool kPair>
 __device__ __forceinline__ void tmem_alloc(uint32_t dst, uint32_t cols) {
-  asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(dst), "r"(cols) : "memory");
-  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  if constexpr (kPair) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(dst), "r"(cols) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  } else {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(dst), "r"(cols) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
 }
+template <bool kPair>
 __device__ __forceinline__ void tmem_free(uint32_t addr, uint32_t cols) {
-  asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(addr), "r"(cols) : "memory");
+  if constexpr (kPair)
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(addr), "r"(cols) : "memory");
+  else
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(addr), "r"(cols) : "memory");
 }
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-// d (+)= A B over 16 elements of k, bf16 or f16 operands in shared memory.
+// d (+)= A B over 16 elements of k, bf16 operands in shared memory.
+template <bool kPair>
 __device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
-  asm volatile(
-      "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add)
-      : "memory");
+  if constexpr (kPair)
+    asm volatile(
+        "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add)
+        : "memory");
+  else
+    asm volatile(
+        "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add)
+        : "memory");
 }
-// Arrives on `bar` once every MMA issued so far by this thread is done.
+// Arrives on `bar` (kPair: of both CTAs) once every MMA issued so far by
+// this thread is done.
+template <bool kPair>
 __device__ __forceinline__ void mma_commit(uint32_t bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+  if constexpr (kPair)
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
+                 "h"((uint16_t)3)
+                 : "memory");
+  else
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
 // 32 consecutive accumulator columns of this thread's lane.
 __device__ __forceinline__ void tmem_load32(uint32_t addr, float (&v)[32]) {
@@ -125,9 +188,9 @@ __device__ __forceinline__ uint64_t tile_desc(uint32_t at, bool mn_major) {
   return (uint64_t)((at >> 4) & 0x3fffu) | lead << 16 | stride << 32 | 1ull << 46 | 2ull << 61;
 }
 __device__ __forceinline__ uint32_t k_step(bool mn_major) { return mn_major ? 2048u >> 4 : 32u >> 4; }
-// f32 accumulators, bf16 operands, 128 x n.
-__device__ __forceinline__ uint32_t instr_desc(int n, bool a_mn, bool b_mn) {
-  return 1u << 4 | 1u << 7 | 1u << 10 | (uint32_t)a_mn << 15 | (uint32_t)b_mn << 16 | (uint32_t)(n >> 3) << 17 | (128u >> 4) << 24;
+// f32 accumulators, bf16 operands, m x n.
+__device__ __forceinline__ uint32_t instr_desc(int m, int n, bool a_mn, bool b_mn) {
+  return 1u << 4 | 1u << 7 | 1u << 10 | (uint32_t)a_mn << 15 | (uint32_t)b_mn << 16 | (uint32_t)(n >> 3) << 17 | (uint32_t)(m >> 4) << 24;
 }
 
 __device__ __forceinline__ float exp2_fast(float v) {

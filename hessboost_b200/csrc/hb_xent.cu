@@ -102,22 +102,30 @@ Operand operand_of(const Sizes& z, int32_t dtype, const void* p, uint64_t stride
   return {packed, packed ? round_up(2ull * z.planes * rows * z.padded, 256) : 0};
 }
 
-// Columns of a tile: 256 where there are enough of them and enough tiles
-// for the SMs, else fewer (in steps of 64).
-int tile_cols(uint64_t cols, uint64_t m_tiles, int sms) {
-  int n = cols >= 256 ? 256 : (int)round_up(cols, 64);
-  while (n > 64 && m_tiles * ((cols + n - 1) / n) < (uint64_t)sms) n = n > 128 ? 128 : 64;
-  return n;
+// Whether pairs of CTAs (256-row tiles) do the work: where rows, classes and
+// width fill such tiles, and enough of them for every pair.
+bool use_pairs(uint64_t rows, uint64_t classes, uint32_t width, int sms) {
+  return rows >= 256 && classes >= 256 && width >= 128 && ((rows + 255) / 256) * ((classes + 255) / 256) >= (uint64_t)sms / 2;
 }
-// Parts of k: enough tiles for the SMs, at least 4 steps of 64 each.
-int k_splits(uint64_t tiles, int k_blocks, int sms) {
-  if (tiles >= (uint64_t)sms) return 1;
-  const int want = (int)((sms + tiles - 1) / tiles);
+
+// Columns of a tile: as few whole tiles of at most 256 as there need be, all
+// alike (multiples of `unit`), or narrower ones where there are not enough
+// tiles for the workers.
+int tile_cols(uint64_t cols, uint64_t m_tiles, int workers, int unit) {
+  uint64_t n = (cols + 255) / 256;
+  while (m_tiles * n < (uint64_t)workers && (cols + n) / (n + 1) > 64) ++n;
+  return (int)round_up((cols + n - 1) / n, unit);
+}
+// Parts of k: enough tiles for the workers, at least 4 steps of 64 each.
+int k_splits(uint64_t tiles, int k_blocks, int workers) {
+  if (tiles >= (uint64_t)workers) return 1;
+  const int want = (int)((workers + tiles - 1) / tiles);
   return std::max(1, std::min(want, k_blocks / 4));
 }
 
 struct Forward {
   Operand x, w;
+  bool pair;
   int n_size, n_tiles;
   uint64_t chunk, part, at_label, bytes;
 };
@@ -125,9 +133,11 @@ Forward forward_plan(const Sizes& z, int32_t dtype, const void* x, uint64_t x_st
   Forward f;
   f.x = operand_of(z, dtype, x, x_stride, z.n_rows, false);
   f.w = operand_of(z, dtype, w, w_stride, z.n_classes, false);
-  f.n_size = tile_cols(z.n_classes, (z.n_rows + 127) / 128, sms);
+  f.pair = use_pairs(z.n_rows, z.n_classes, z.width, sms);
+  const int m = f.pair ? 256 : 128;
+  f.n_size = tile_cols(z.n_classes, (z.n_rows + m - 1) / m, f.pair ? sms / 2 : sms, f.pair ? 128 : 64);
   f.n_tiles = (int)((z.n_classes + f.n_size - 1) / f.n_size);
-  f.chunk = std::min<uint64_t>(z.n_rows, std::max<uint64_t>(128, kPartBytes / (8ull * f.n_tiles) / 128 * 128));
+  f.chunk = std::min<uint64_t>(z.n_rows, std::max<uint64_t>(256, kPartBytes / (8ull * f.n_tiles) / 256 * 256));
   f.part = round_up(8ull * f.n_tiles * f.chunk, 256);
   f.at_label = round_up(4 * f.chunk, 256);
   f.bytes = f.x.bytes + f.w.bytes + f.part + f.at_label;
@@ -136,6 +146,7 @@ Forward forward_plan(const Sizes& z, int32_t dtype, const void* x, uint64_t x_st
 
 struct Backward {
   Operand x, w;
+  bool pair;
   uint64_t piece, chunk, pieces, chunks;
   uint64_t g_stride;                      // elements of a row of G
   int grad_n, out_n;                      // tile columns of grad, and of dx and dw
@@ -143,7 +154,7 @@ struct Backward {
   bool dx_acc, dw_acc;
   uint32_t acc_stride;
   uint64_t dw_rows;                       // rows of a dw accumulator
-  uint64_t g_bytes, dx_bytes, dw_bytes, bytes;
+  uint64_t g_bytes, dx_bytes, dw_bytes, bytes;  // g_bytes of one piece: there are two where there are two pieces
 };
 Backward backward_plan(const Sizes& z, int32_t dtype, const void* x, uint64_t x_stride, const void* w, uint64_t w_stride, int sms) {
   Backward b;
@@ -151,18 +162,20 @@ Backward backward_plan(const Sizes& z, int32_t dtype, const void* x, uint64_t x_
   b.w = operand_of(z, dtype, w, w_stride, z.n_classes, false);
   const uint64_t most = (uint64_t)kGradElements / z.planes;
   const uint64_t least = 4096;  // classes of a piece, where there are as many
-  b.chunk = std::min(z.n_rows, std::max<uint64_t>(most / std::min(z.n_classes, least) / 128 * 128, 128));
+  b.chunk = std::min(z.n_rows, std::max<uint64_t>(most / std::min(z.n_classes, least) / 256 * 256, 256));
   b.chunks = (z.n_rows + b.chunk - 1) / b.chunk;
   b.piece = std::min(z.n_classes, std::max<uint64_t>(most / b.chunk / 256 * 256, 256));
   b.pieces = (z.n_classes + b.piece - 1) / b.piece;
   b.piece = std::min(b.piece, round_up((z.n_classes + b.pieces - 1) / b.pieces, 256));
+  b.pair = use_pairs(b.chunk, b.piece, z.width, sms);
+  const int m = b.pair ? 256 : 128, workers = b.pair ? sms / 2 : sms;
   b.g_stride = round_up(b.piece, 64);
-  const uint64_t row_tiles = (b.chunk + 127) / 128, class_tiles = (b.piece + 127) / 128;
-  b.grad_n = tile_cols(b.piece, row_tiles, sms);
-  b.out_n = tile_cols(z.width, row_tiles + class_tiles, sms);
+  const uint64_t row_tiles = (b.chunk + m - 1) / m, class_tiles = (b.piece + m - 1) / m;
+  b.grad_n = tile_cols(b.piece, row_tiles, workers, b.pair ? 128 : 64);
+  b.out_n = tile_cols(z.width, row_tiles + class_tiles, workers, 32);
   const uint64_t out_tiles = (z.width + b.out_n - 1) / b.out_n;
-  b.dx_splits = k_splits(row_tiles * out_tiles, (int)((b.piece + 63) / 64), sms);
-  b.dw_splits = k_splits(class_tiles * out_tiles, (int)((b.chunk + 63) / 64), sms);
+  b.dx_splits = k_splits(row_tiles * out_tiles, (int)((b.piece + 63) / 64), workers);
+  b.dw_splits = k_splits(class_tiles * out_tiles, (int)((b.chunk + 63) / 64), workers);
   b.dx_acc = b.dx_splits > 1 || b.pieces > 1;
   b.dw_acc = b.dw_splits > 1 || b.chunks > 1;
   b.acc_stride = (uint32_t)round_up(z.width, 4);
@@ -170,7 +183,7 @@ Backward backward_plan(const Sizes& z, int32_t dtype, const void* x, uint64_t x_
   b.g_bytes = round_up(2ull * z.planes * b.chunk * b.g_stride, 256);
   b.dx_bytes = b.dx_acc ? round_up(4ull * b.dx_splits * b.chunk * b.acc_stride, 256) : 0;
   b.dw_bytes = b.dw_acc ? round_up(4ull * b.dw_splits * b.dw_rows * b.acc_stride, 256) : 0;
-  b.bytes = b.x.bytes + b.w.bytes + b.g_bytes + b.dx_bytes + b.dw_bytes;
+  b.bytes = b.x.bytes + b.w.bytes + (b.pieces * b.chunks > 1 ? 2 : 1) * b.g_bytes + b.dx_bytes + b.dw_bytes;
   return b;
 }
 
@@ -265,23 +278,21 @@ hb_status hb_linear_xent_forward(int32_t device, const void* x, uint64_t x_strid
   p.at_label = (float*)(at + f.part);
   p.pairs = z.planes == 3 ? 6 : 1;
   p.planes = z.planes;
-  p.n_classes = (int)n_classes;
   p.all_classes = (int64_t)n_classes;
   p.width = (int)width;
+  p.labels = labels;
   p.label_type = label_type;
   p.n_jobs = 1;
-  const uint64_t label_size = label_type == HB_I32 ? 4 : 8;
+  const int m = f.pair ? 256 : 128;
   for (uint64_t r0 = 0; r0 < n_rows; r0 += f.chunk) {
     const uint64_t rows = std::min(f.chunk, n_rows - r0);
-    p.n_rows = (int)rows;
-    p.row0 = (int)r0;
-    p.labels = (const char*)labels + r0 * label_size;
     p.part_stride = rows;
-    p.jobs[0] = MmaJob{kJobStats, 0, (int)((rows + 127) / 128), f.n_tiles, f.n_size, (int)((width + 63) / 64), 1, 1, {}};
-    if (hb_status st = mma_launch(p, sms, s)) return st;
+    p.jobs[0] = MmaJob{kJobStats, (int)((rows + m - 1) / m), f.n_tiles, f.n_size, (int)((width + 63) / 64), 1, 1,
+                       (int)r0, (int)rows, 0, (int)n_classes, {}};
+    if (hb_status st = mma_launch(p, f.pair, sms, s)) return st;
     with_xent_types(dtype, label_type, [&](auto, auto l) {
       using L = decltype(l);
-      k_xent_join<L><<<(int)((rows + 255) / 256), 256, 0, s>>>(p.part, f.n_tiles, p.at_label, (const L*)p.labels, rows, n_classes,
+      k_xent_join<L><<<(int)((rows + 255) / 256), 256, 0, s>>>(p.part, f.n_tiles, p.at_label, (const L*)labels + r0, rows, n_classes,
                                                            loss + r0, lse + r0);
     });
   }
@@ -330,20 +341,24 @@ hb_status hb_linear_xent_backward(int32_t device, const float* dloss, uint64_t d
       !operand(&p.w, b.w, z, dtype, w, w_stride, n_classes, nullptr, label_type, at + b.x.bytes, sms, s))
     return fail(HB_DEVICE_FAILED, "tensor map");
   at += b.x.bytes + b.w.bytes;
-  void* g = at;
-  float* dx_acc = (float*)(at + b.g_bytes);
-  float* dw_acc = (float*)(at + b.g_bytes + b.dx_bytes);
+  const uint64_t steps = b.chunks * b.pieces;
+  char* const g[2] = {at, steps > 1 ? at + b.g_bytes : at};
+  at = g[1] + b.g_bytes;
+  float* dx_acc = (float*)at;
+  float* dw_acc = (float*)(at + b.dx_bytes);
   p.pairs = z.planes == 3 ? 6 : 1;
   p.planes = z.planes;
   p.all_classes = (int64_t)n_classes;
   p.width = (int)width;
+  p.labels = labels;
   p.label_type = label_type;
+  p.dloss = dloss;
   p.dloss_stride = dloss_stride;
-  p.first_dloss = dloss;
-  const uint64_t label_size = label_type == HB_I32 ? 4 : 8, e = size_of(dtype);
-  const int out_type = dtype == HB_F32 ? kOutF32 : kOutBf16;
+  p.lse = lse;
+  const uint64_t e = size_of(dtype);
+  const int out_type = dtype == HB_F32 ? kOutF32 : kOutBf16, m = b.pair ? 256 : 128;
   const int out_tiles = (int)((width + b.out_n - 1) / b.out_n);
-  const auto vec = [&](const void* q) { return (int)(aligned(q, 16) && width * e % 16 == 0); };
+  const auto vec = [&](const void* q) { return (int)(aligned(q, 16) && width * e % 16 == 0 && b.out_n * e % 16 == 0); };
   // dx or dw of `rows` rows from `splits` accumulators
   const auto finish = [&](const float* acc, int splits, uint64_t split_rows, uint64_t rows, void* to) {
     const int grid = grid_for(rows * width, kFinishThreads, sms);
@@ -352,39 +367,50 @@ hb_status hb_linear_xent_backward(int32_t device, const float* dloss, uint64_t d
     else
       k_xent_finish<__nv_bfloat16><<<grid, kFinishThreads, 0, s>>>(acc, splits, split_rows, rows, width, b.acc_stride, (__nv_bfloat16*)to);
   };
-  for (uint64_t c = 0; c < b.chunks; ++c) {
-    const uint64_t r0 = c * b.chunk, rows = std::min(b.chunk, n_rows - r0);
-    void* dx_to = (char*)dx + r0 * width * e;
-    p.n_rows = (int)rows;
-    p.row0 = (int)r0;
-    p.labels = (const char*)labels + r0 * label_size;
-    p.dloss = dloss + r0 * dloss_stride;
-    p.lse = lse + r0;
-    for (uint64_t q = 0; q < b.pieces; ++q) {
-      const uint64_t v0 = q * b.piece, classes = std::min(b.piece, n_classes - v0);
-      void* dw_to = (char*)dw + v0 * width * e;
-      p.n_classes = (int)classes;
-      p.class0 = (int)v0;
-      if (!mma_map(&p.g, g, classes, rows, z.planes, b.g_stride, b.chunk * b.g_stride, 64) ||
-          !mma_map(&p.g_out, g, classes, rows, z.planes, b.g_stride, b.chunk * b.g_stride, 32))
-        return fail(HB_DEVICE_FAILED, "tensor map");
-      const int row_tiles = (int)((rows + 127) / 128), class_tiles = (int)((classes + 127) / 128);
-      p.n_jobs = 1;
-      p.jobs[0] = MmaJob{kJobGrad, 0, row_tiles, (int)((classes + b.grad_n - 1) / b.grad_n), b.grad_n, (int)((width + 63) / 64), 1, 1, {}};
-      if (hb_status st = mma_launch(p, sms, s)) return st;
-      const int class_blocks = (int)((classes + 63) / 64), row_blocks = (int)((rows + 63) / 64);
-      MmaOut to_dx{b.dx_acc ? kOutAcc : out_type, q > 0, vec(dx_to), (int)b.chunk, (int)b.acc_stride, dx_acc, dx_to};
-      float* acc = b.chunks > 1 ? dw_acc + v0 * b.acc_stride : dw_acc;
-      MmaOut to_dw{b.dw_acc ? kOutAcc : out_type, c > 0, vec(dw_to), (int)b.dw_rows, (int)b.acc_stride, acc, dw_to};
-      // a last piece or chunk may have fewer steps than splits: the splits
-      // past them add nothing, and are not read
-      p.n_jobs = 2;
-      p.jobs[0] = MmaJob{kJobDw, 0, class_tiles, out_tiles, b.out_n, row_blocks, b.dw_splits, 0, to_dw};
-      p.jobs[1] = MmaJob{kJobDx, 0, row_tiles, out_tiles, b.out_n, class_blocks, b.dx_splits, 0, to_dx};
-      if (hb_status st = mma_launch(p, sms, s)) return st;
-      if (b.dw_acc && c + 1 == b.chunks) finish(acc, b.dw_splits, b.dw_rows, classes, dw_to);
+  // Step i is piece i mod pieces of chunk i / pieces. A launch takes dw and
+  // dx of one step's G and forms the next step's, whose small tiles fill up
+  // the workers that the large ones leave uneven.
+  for (uint64_t i = 0; i <= steps; ++i) {
+    p.n_jobs = 0;
+    const auto sizes = [&](MmaJob& job, uint64_t step) {
+      const uint64_t r0 = step / b.pieces * b.chunk, v0 = step % b.pieces * b.piece;
+      job.row0 = (int)r0, job.n_rows = (int)std::min(b.chunk, n_rows - r0);
+      job.class0 = (int)v0, job.n_classes = (int)std::min(b.piece, n_classes - v0);
+    };
+    const auto g_map = [&](CUtensorMap* map, const MmaJob& job, uint64_t step, int box_rows) {
+      return mma_map(map, g[step & 1], job.n_classes, job.n_rows, z.planes, b.g_stride, b.chunk * b.g_stride, box_rows);
+    };
+    MmaJob done{};
+    void *dx_to = nullptr, *dw_to = nullptr;
+    float* acc = nullptr;
+    const uint64_t c = (i - 1) / b.pieces, q = (i - 1) % b.pieces;  // of the step done, where i > 0
+    if (i > 0) {
+      sizes(done, i - 1);
+      if (!g_map(&p.g, done, i - 1, 64)) return fail(HB_DEVICE_FAILED, "tensor map");
+      dx_to = (char*)dx + (uint64_t)done.row0 * width * e;
+      dw_to = (char*)dw + (uint64_t)done.class0 * width * e;
+      acc = b.chunks > 1 ? dw_acc + (uint64_t)done.class0 * b.acc_stride : dw_acc;
+      // a last piece or chunk may have fewer steps of k than splits: the
+      // splits without any add 0
+      MmaJob& jw = p.jobs[p.n_jobs++] = done;
+      jw.kind = kJobDw, jw.m_tiles = (done.n_classes + m - 1) / m, jw.n_tiles = out_tiles, jw.n_size = b.out_n;
+      jw.k_blocks = (done.n_rows + 63) / 64, jw.splits = b.dw_splits;
+      jw.out = MmaOut{b.dw_acc ? kOutAcc : out_type, c > 0, vec(dw_to), (int)b.dw_rows, (int)b.acc_stride, acc, dw_to};
+      MmaJob& jx = p.jobs[p.n_jobs++] = done;
+      jx.kind = kJobDx, jx.m_tiles = (done.n_rows + m - 1) / m, jx.n_tiles = out_tiles, jx.n_size = b.out_n;
+      jx.k_blocks = (done.n_classes + 63) / 64, jx.splits = b.dx_splits;
+      jx.out = MmaOut{b.dx_acc ? kOutAcc : out_type, q > 0, vec(dx_to), (int)b.chunk, (int)b.acc_stride, dx_acc, dx_to};
     }
-    if (b.dx_acc) finish(dx_acc, b.dx_splits, b.chunk, rows, dx_to);
+    if (i < steps) {
+      MmaJob& jg = p.jobs[p.n_jobs++] = MmaJob{};
+      sizes(jg, i);
+      if (!g_map(&p.g_out, jg, i, 32)) return fail(HB_DEVICE_FAILED, "tensor map");
+      jg.kind = kJobGrad, jg.m_tiles = (jg.n_rows + m - 1) / m, jg.n_tiles = (jg.n_classes + b.grad_n - 1) / b.grad_n;
+      jg.n_size = b.grad_n, jg.k_blocks = (int)((width + 63) / 64), jg.splits = 1, jg.m_fast = 1;
+    }
+    if (hb_status st = mma_launch(p, b.pair, sms, s)) return st;
+    if (i > 0 && b.dw_acc && c + 1 == b.chunks) finish(acc, b.dw_splits, b.dw_rows, done.n_classes, dw_to);
+    if (i > 0 && b.dx_acc && q + 1 == b.pieces) finish(dx_acc, b.dx_splits, b.chunk, done.n_rows, dx_to);
   }
   return launched("hb_linear_xent_backward");
 }

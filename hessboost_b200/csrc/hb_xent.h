@@ -22,34 +22,39 @@ struct MmaOut {
   void* to;
 };
 
-// m_tiles x n_tiles tiles of 128 x n_size, k in steps of 64 shared among
-// `splits` tiles each; m_fast: consecutive tiles go down the rows.
+// m_tiles x n_tiles tiles of (128 x CTAs) x n_size, k in steps of 64 shared
+// among `splits` tiles each; m_fast: consecutive tiles go down the rows.
+// The job's rows are [row0, row0 + n_rows) of the call's, its classes
+// [class0, class0 + n_classes) of the layer's.
 struct MmaJob {
-  int kind, tiles, m_tiles, n_tiles, n_size, k_blocks, splits, m_fast;
+  int kind, m_tiles, n_tiles, n_size, k_blocks, splits, m_fast;
+  int row0, n_rows, class0, n_classes;
   MmaOut out;
 };
 
+constexpr int kMaxJobs = 3;
+constexpr int kMaxWorkers = 160;
+
 struct MmaParams {
-  CUtensorMap x, w, g, g_out;  // bf16 [planes][rows][columns]
-  MmaJob jobs[3];
-  int n_jobs, tiles;
+  CUtensorMap x, w, g, g_out;  // bf16 [planes][rows][columns]; dx and dw read g, grad writes g_out
+  MmaJob jobs[kMaxJobs];
+  int n_jobs;
   int pairs, planes;           // 1, 1: bf16; 6, 3: f32 in three pieces
-  int n_rows, n_classes, width;  // of this launch: the chunk's rows, the piece's classes
-  int row0, class0;            // the chunk's first row in x, the piece's first class in w
-  // of the chunk's rows
-  const void* labels;
+  int width;
+  const void* labels;          // of the call's rows, as the next three
   int label_type;
   int64_t all_classes;
-  const float* first_dloss;    // of the call's first row
   const float* dloss;
   uint64_t dloss_stride;
   const float* lse;
   float2* part;                // stats: [n_tiles][part_stride]
   uint64_t part_stride;
-  float* at_label;
+  float* at_label;             // stats: of the job's rows
+  // worker u (a CTA, or a pair) takes tiles [first[j][u], first[j][u + 1]) of job j
+  int first[kMaxJobs][kMaxWorkers + 1];
 
   // The row's label, -1 where it has none.
-  __device__ __forceinline__ int64_t label(int row) const {
+  __device__ __forceinline__ int64_t label(int64_t row) const {
     const int64_t v = label_type == HB_I32 ? (int64_t)((const int32_t*)labels)[row] : ((const int64_t*)labels)[row];
     return v >= 0 && v < all_classes ? v : -1;
   }
@@ -59,8 +64,8 @@ struct MmaParams {
 // elements, multiples of 8, the address 16-byte aligned.
 bool mma_map(CUtensorMap* map, const void* p, uint64_t cols, uint64_t rows, uint64_t planes, uint64_t row_stride,
              uint64_t plane_stride, int box_rows);
-// Runs the jobs; fills in the tile counts.
-hb_status mma_launch(MmaParams& p, int sms, cudaStream_t s);
+// Runs the jobs by single CTAs or (pair) by pairs of them; shares the tiles out.
+hb_status mma_launch(MmaParams& p, bool pair, int sms, cudaStream_t s);
 
 }  // namespace head
 }  // namespace hb

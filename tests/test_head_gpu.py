@@ -392,6 +392,28 @@ def test_xent(head, dtype, n, d, v):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("n,d,v", [(2500, 136, 2600), (4999, 520, 1300), (3000, 257, 9000), (60000, 24, 1000), (20000, 160, 6000),
+                                   (9000, 72, 5000)])
+def test_xent_pieces_and_chunks(head, dtype, n, d, v):
+    # several pieces of the classes, chunks of the rows, both; tiles of one CTA and of two
+    check_xent(head, *xent_inputs(gen(n + d + v), n, d, v, dtype))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_xent_one_factor_for_all_rows(head, dtype):
+    # a mean's factor, whose rounding to the inputs' type would be the same for every row: 1 / 1000 is 2.2e-3 off in bf16
+    x, w, labels, _ = xent_inputs(gen(25), 1000, 64, 500, dtype)
+    labels[0] = 3
+    dl = torch.full((1000,), 1e-3, device="cuda")
+    _, lse = head.linear_xent_forward(x, w, labels)
+    dx, dw = head.linear_xent_backward(dl, x, w, labels, lse)
+    r = xent64(x, w, labels, dl)
+    # one rounding of the output, and one of random size of each element of G
+    assert float((dx.double() - r["dx"]).norm() / r["dx"].norm()) <= 0.75 * UNIT[dtype] + 64 * U
+    assert float((dw.double() - r["dw"]).norm() / r["dw"].norm()) <= 0.75 * UNIT[dtype] + 64 * U
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("n,d,v", [(40, 64, 12), (200, 96, 3000)])
 def test_xent_large_logits(head, dtype, n, d, v):
     # logits of hundreds: peaked rows, where exp of the plain logit overflows
