@@ -80,22 +80,22 @@ __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile
 // ---- TMA -----------------------------------------------------------------
 // kPair: `bar` may be the pair's other CTA's.
 template <bool kPair>
-__device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y, int z) {
+__device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y, int z, int u) {
   if constexpr (kPair)
     asm volatile(
-        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%3, %4, %5}], "
+        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%3, %4, %5, %6}], "
         "[%2];" ::"r"(dst),
-        "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z)
+        "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z), "r"(u)
         : "memory");
   else
     asm volatile(
-        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst),
-        "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z)
+        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst),
+        "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z), "r"(u)
         : "memory");
 }
-__device__ __forceinline__ void tma_store(const CUtensorMap* map, uint32_t src, int x, int y, int z) {
-  asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(map), "r"(src), "r"(x),
-               "r"(y), "r"(z)
+__device__ __forceinline__ void tma_store(const CUtensorMap* map, uint32_t src, int x, int y, int z, int u) {
+  asm volatile("cp.async.bulk.tensor.4d.global.shared::cta.tile.bulk_group [%0, {%2, %3, %4, %5}], [%1];" ::"l"(map), "r"(src), "r"(x),
+               "r"(y), "r"(z), "r"(u)
                : "memory");
 }
 __device__ __forceinline__ void tma_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
@@ -174,17 +174,17 @@ __device__ __forceinline__ void tmem_load32(uint32_t addr, float (&v)[32]) {
   for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
 }
 
-// Shared-memory operand descriptors of tiles made of 64 x 64 blocks of
-// 16-bit elements (8 KiB each: 64 rows of 128 bytes, 128-byte swizzle, as a
-// TMA box {64, 64} writes them), `at` the tile's address.
-//   k-major  (a row of the block is one row of the operand, its 128 bytes 64
-//            elements of k): 8-row groups 1,024 bytes apart; the next 16 of
-//            k start 32 bytes on
-//   mn-major (a row of the block is one k, its 128 bytes 64 operand rows):
-//            8-k groups 1,024 bytes apart, the next 64 operand rows one block
-//            (8,192 bytes) on; the next 16 of k start 2,048 bytes on
-__device__ __forceinline__ uint64_t tile_desc(uint32_t at, bool mn_major) {
-  const uint64_t lead = mn_major ? 8192u >> 4 : 1u, stride = 1024u >> 4;
+// Shared-memory operand descriptors of 16-bit tiles in blocks of 64 columns
+// (a row of a block is 128 bytes, swizzled over 8 rows, as a TMA box 64
+// columns wide writes it), `at` the tile's address, a multiple of 1,024.
+//   k-major  (a block's rows are the operand's, its columns 64 of k): groups
+//            of 8 rows 1,024 bytes apart; the next 16 of k start 32 bytes on
+//   mn-major (a block's rows are k, its columns 64 of the operand's rows):
+//            groups of 8 of k 1,024 bytes apart, the next 64 of the operand's
+//            rows one block (`k_rows` rows) on; the next 16 of k start 2,048
+//            bytes on
+__device__ __forceinline__ uint64_t tile_desc(uint32_t at, bool mn_major, uint32_t k_rows) {
+  const uint64_t lead = mn_major ? k_rows * 128u >> 4 : 1u, stride = 1024u >> 4;
   return (uint64_t)((at >> 4) & 0x3fffu) | lead << 16 | stride << 32 | 1ull << 46 | 2ull << 61;
 }
 __device__ __forceinline__ uint32_t k_step(bool mn_major) { return mn_major ? 2048u >> 4 : 32u >> 4; }

@@ -30,54 +30,104 @@ __device__ __forceinline__ int64_t label_of(const L* labels, uint64_t r, uint64_
 // x in bf16 pieces, out[plane][row][padded], zero past `width`; where labels
 // are given, rows without one are zero (whatever they hold, a product with
 // their zero row of G is to add nothing).
+// A thread makes 8 columns of a row.
 template <typename T, typename L, int kPlanes>
 __global__ void k_xent_pack(const T* __restrict__ x, uint64_t x_stride, uint64_t n_rows, uint32_t width,
-                            uint32_t padded, const L* __restrict__ labels, uint64_t n_classes,
+                            uint32_t padded, int vec, const L* __restrict__ labels, uint64_t n_classes,
                             __nv_bfloat16* __restrict__ out) {
-  const uint64_t total = n_rows * padded;
+  const uint32_t groups = padded / 8;
+  const uint64_t total = n_rows * groups;
   for (uint64_t i = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (uint64_t)gridDim.x * blockDim.x) {
-    const uint64_t r = i / padded;
-    const uint32_t d = (uint32_t)(i - r * padded);
-    float v = 0.0f;
-    if (d < width && (!labels || label_of(labels, r, n_classes) >= 0)) v = to_f32(x[r * x_stride + d]);
+    const uint64_t r = total >> 32 ? i / groups : (uint32_t)i / groups;
+    const uint32_t d = (uint32_t)(i - r * groups) * 8;
+    float v[8] = {};
+    if (d < width && (!labels || label_of(labels, r, n_classes) >= 0)) {
+      const T* from = x + r * x_stride + d;
+      if (vec && d + 8 <= width) {
+        constexpr int kPer = 16 / sizeof(T);
+#pragma unroll
+        for (int j = 0; j < 8; j += kPer) {
+          const Pack<T, kPer> q = *reinterpret_cast<const Pack<T, kPer>*>(from + j);
+#pragma unroll
+          for (int k = 0; k < kPer; ++k) v[j + k] = to_f32(q.v[k]);
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (d + j < width) v[j] = to_f32(from[j]);
+      }
+    }
 #pragma unroll
     for (int q = 0; q < kPlanes; ++q) {
-      const __nv_bfloat16 b = __float2bfloat16_rn(v);
-      out[q * total + i] = b;
-      if (q + 1 < kPlanes) v -= __bfloat162float(b);
+      Pack<__nv_bfloat16, 8> b;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        b.v[j] = __float2bfloat16_rn(v[j]);
+        if (q + 1 < kPlanes) v[j] -= __bfloat162float(b.v[j]);
+      }
+      *reinterpret_cast<Pack<__nv_bfloat16, 8>*>(out + (q * n_rows + r) * padded + d) = b;
     }
   }
 }
 
-// Joins the tiles' (max, sum) of each row in class order.
+// Joins the tiles' (max, sum) of each row: a CTA's 32 rows, each warp its
+// share of the tiles in class order, then the warps in theirs.
+constexpr int kJoinWarps = 16;
+__device__ __forceinline__ float2 joined(float2 a, float2 b) {
+  const float top = fmaxf(a.x, b.x);
+  a.y = (a.x == top ? a.y : a.y * expf(a.x - top)) + (b.x == top ? b.y : b.y * expf(b.x - top));
+  // a NaN maximum (a product that gave up) stays
+  a.x = a.x != a.x || b.x != b.x ? NAN : top;
+  return a;
+}
 template <typename L>
-__global__ void k_xent_join(const float2* __restrict__ part, int parts, const float* __restrict__ at_label,
-                            const L* __restrict__ labels, uint64_t n_rows, uint64_t n_classes,
-                            float* __restrict__ loss, float* __restrict__ lse) {
-  const uint64_t r = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x;
-  if (r >= n_rows) return;
-  float2 a = part[r];
-  for (int i = 1; i < parts; ++i) {
-    const float2 b = part[(uint64_t)i * n_rows + r];
-    const float top = fmaxf(a.x, b.x);
-    a.y = (a.x == top ? a.y : a.y * expf(a.x - top)) + (b.x == top ? b.y : b.y * expf(b.x - top));
-    a.x = top;
+__global__ void __launch_bounds__(32 * kJoinWarps)
+    k_xent_join(const float2* __restrict__ part, int parts, const float* __restrict__ at_label,
+                const L* __restrict__ labels, uint64_t n_rows, uint64_t n_classes, float* __restrict__ loss,
+                float* __restrict__ lse) {
+  __shared__ float2 sh[kJoinWarps][32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const uint64_t r = (uint64_t)blockIdx.x * 32 + lane;
+  float2 a = make_float2(-INFINITY, 0.0f);
+  if (r < n_rows) {
+    const int p0 = parts * warp / kJoinWarps, p1 = parts * (warp + 1) / kJoinWarps;
+#pragma unroll 8
+    for (int i = p0; i < p1; ++i) a = joined(a, part[(uint64_t)i * n_rows + r]);
   }
+  sh[warp][lane] = a;
+  __syncthreads();
+  if (warp || r >= n_rows) return;
+  for (int i = 1; i < kJoinWarps; ++i) a = joined(a, sh[i][lane]);
   const float l = a.x + logf(a.y);
   lse[r] = l;
   loss[r] = label_of(labels, r, n_classes) >= 0 ? l - at_label[r] : 0.0f;
 }
 
-// out[r][d] = the sum of the splits' accumulators, in their order.
+// out[r][d] = the sum of the splits' accumulators, in their order; a thread
+// makes 4 columns of a row.
 template <typename T>
 __global__ void k_xent_finish(const float* __restrict__ acc, int splits, uint64_t split_rows, uint64_t n_rows,
-                              uint32_t width, uint32_t acc_stride, T* __restrict__ out) {
-  const uint64_t total = n_rows * width;
+                              uint32_t width, uint32_t acc_stride, int vec, T* __restrict__ out) {
+  const uint32_t groups = acc_stride / 4;
+  const uint64_t total = n_rows * groups;
   for (uint64_t i = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (uint64_t)gridDim.x * blockDim.x) {
-    const uint64_t r = i / width, at = r * acc_stride + (i - r * width);
-    float v = acc[at];
-    for (int s = 1; s < splits; ++s) v += acc[s * split_rows * acc_stride + at];
-    out[i] = from_f32<T>(v);
+    const uint64_t r = total >> 32 ? i / groups : (uint32_t)i / groups;
+    const uint32_t d = (uint32_t)(i - r * groups) * 4;
+    const float* from = acc + r * acc_stride + d;
+    float4 v = *reinterpret_cast<const float4*>(from);
+#pragma unroll 4
+    for (int s = 1; s < splits; ++s) {
+      const float4 u = *reinterpret_cast<const float4*>(from + s * split_rows * acc_stride);
+      v.x += u.x, v.y += u.y, v.z += u.z, v.w += u.w;
+    }
+    T* to = out + r * width + d;
+    const T q[4] = {from_f32<T>(v.x), from_f32<T>(v.y), from_f32<T>(v.z), from_f32<T>(v.w)};
+    if (vec) {
+      *reinterpret_cast<Pack<T, 4>*>(to) = Pack<T, 4>{{q[0], q[1], q[2], q[3]}};
+    } else {
+      for (int j = 0; j < 4; ++j)
+        if (d + j < width) to[j] = q[j];
+    }
   }
 }
 
@@ -93,12 +143,12 @@ struct Sizes {
 };
 
 Sizes sizes_of(int32_t dtype, uint64_t n_rows, uint32_t width, uint64_t n_classes) {
-  return {n_rows, n_classes, width, (uint32_t)round_up(width, 8), dtype == HB_F32 ? 3 : 1};
+  return {n_rows, n_classes, width, (uint32_t)round_up(width, 64), dtype == HB_F32 ? 3 : 1};
 }
-// TMA takes bf16 rows as they are where the address and the row stride are
-// whole 16-byte units.
+// bf16 rows of whole 64-column blocks are read as they lie where the address
+// and the row stride are whole 16-byte units, as TMA wants them.
 Operand operand_of(const Sizes& z, int32_t dtype, const void* p, uint64_t stride, uint64_t rows, bool always) {
-  const bool packed = always || dtype != HB_BF16 || !aligned(p, 16) || stride % 8;
+  const bool packed = always || dtype != HB_BF16 || !aligned(p, 16) || stride % 8 || z.width % 64;
   return {packed, packed ? round_up(2ull * z.planes * rows * z.padded, 256) : 0};
 }
 
@@ -108,19 +158,23 @@ bool use_pairs(uint64_t rows, uint64_t classes, uint32_t width, int sms) {
   return rows >= 256 && classes >= 256 && width >= 128 && ((rows + 255) / 256) * ((classes + 255) / 256) >= (uint64_t)sms / 2;
 }
 
+int stages_of(uint64_t k) { return (int)((k + 64 * kMmaDepth - 1) / (64 * kMmaDepth)); }
 // Columns of a tile: as few whole tiles of at most 256 as there need be, all
 // alike (multiples of `unit`), or narrower ones where there are not enough
 // tiles for the workers.
 int tile_cols(uint64_t cols, uint64_t m_tiles, int workers, int unit) {
   uint64_t n = (cols + 255) / 256;
   while (m_tiles * n < (uint64_t)workers && (cols + n) / (n + 1) > 64) ++n;
-  return (int)round_up((cols + n - 1) / n, unit);
+  const auto size = [&](uint64_t k) { return round_up((cols + k - 1) / k, unit); };
+  // one tile more where that leaves much less of the last one empty
+  if (5 * (n + 1) * size(n + 1) <= 4 * n * size(n)) ++n;
+  return (int)size(n);
 }
 // Parts of k: enough tiles for the workers, at least 4 steps of 64 each.
 int k_splits(uint64_t tiles, int k_blocks, int workers) {
   if (tiles >= (uint64_t)workers) return 1;
   const int want = (int)((workers + tiles - 1) / tiles);
-  return std::max(1, std::min(want, k_blocks / 4));
+  return std::max(1, std::min(want, k_blocks * kMmaDepth / 4));
 }
 
 struct Forward {
@@ -172,10 +226,10 @@ Backward backward_plan(const Sizes& z, int32_t dtype, const void* x, uint64_t x_
   b.g_stride = round_up(b.piece, 64);
   const uint64_t row_tiles = (b.chunk + m - 1) / m, class_tiles = (b.piece + m - 1) / m;
   b.grad_n = tile_cols(b.piece, row_tiles, workers, b.pair ? 128 : 64);
-  b.out_n = tile_cols(z.width, row_tiles + class_tiles, workers, 32);
+  b.out_n = tile_cols(z.width, row_tiles + class_tiles, workers, b.pair ? 128 : 64);
   const uint64_t out_tiles = (z.width + b.out_n - 1) / b.out_n;
-  b.dx_splits = k_splits(row_tiles * out_tiles, (int)((b.piece + 63) / 64), workers);
-  b.dw_splits = k_splits(class_tiles * out_tiles, (int)((b.chunk + 63) / 64), workers);
+  b.dx_splits = k_splits(row_tiles * out_tiles, stages_of(b.piece), workers);
+  b.dw_splits = k_splits(class_tiles * out_tiles, stages_of(b.chunk), workers);
   b.dx_acc = b.dx_splits > 1 || b.pieces > 1;
   b.dw_acc = b.dw_splits > 1 || b.chunks > 1;
   b.acc_stride = (uint32_t)round_up(z.width, 4);
@@ -197,20 +251,29 @@ int grid_for(uint64_t threads, int block, int sms) {
   return (int)std::max<uint64_t>(1, std::min<uint64_t>((threads + block - 1) / block, (uint64_t)sms * 16));
 }
 
-// The operand's map with boxes of 64 rows, after packing it to `at` where
-// that is needed.
-bool operand(CUtensorMap* map, const Operand& o, const Sizes& z, int32_t dtype, const void* p, uint64_t stride, uint64_t rows,
-             const void* labels, int32_t label_type, void* at, int sms, cudaStream_t s) {
-  if (!o.packed) return mma_map(map, p, z.width, rows, 1, stride, stride * rows, 64);
+// The operand as the products read it, after packing it to `at` where that
+// is needed.
+struct Lay {
+  const void* p;
+  uint64_t rows, stride, plane;
+  int planes, blocks;
+  bool map(CUtensorMap* m, int box_rows, int box_blocks) const {
+    return mma_map(m, p, blocks, rows, planes, stride, plane, box_rows, box_blocks);
+  }
+};
+Lay operand(const Operand& o, const Sizes& z, int32_t dtype, const void* p, uint64_t stride, uint64_t rows, const void* labels,
+            int32_t label_type, void* at, int sms, cudaStream_t s) {
+  if (!o.packed) return {p, rows, stride, stride, 1, (int)(z.width / 64)};
   const uint64_t total = rows * z.padded;
   with_xent_types(dtype, label_type, [&](auto t, auto l) {
     using T = decltype(t);
     using L = decltype(l);
     constexpr int kPlanes = sizeof(T) == 4 ? 3 : 1;
-    k_xent_pack<T, L, kPlanes><<<grid_for(total, 256, sms), 256, 0, s>>>((const T*)p, stride, rows, z.width, z.padded,
+    k_xent_pack<T, L, kPlanes><<<grid_for(total / 8, 256, sms), 256, 0, s>>>((const T*)p, stride, rows, z.width, z.padded,
+                                                                   aligned(p, 16) && stride * sizeof(T) % 16 == 0,
                                                                    (const L*)labels, z.n_classes, (__nv_bfloat16*)at);
   });
-  return mma_map(map, at, z.padded, rows, z.planes, z.padded, total, 64);
+  return {at, rows, z.padded, total, z.planes, (int)(z.padded / 64)};
 }
 
 hb_status check_xent(const void* x, uint64_t x_stride, const void* w, uint64_t w_stride, int32_t dtype, uint64_t n_rows,
@@ -270,13 +333,13 @@ hb_status hb_linear_xent_forward(int32_t device, const void* x, uint64_t x_strid
   cudaStream_t s = (cudaStream_t)stream;
   char* at = (char*)workspace;
   MmaParams p{};
-  if (!operand(&p.x, f.x, z, dtype, x, x_stride, n_rows, nullptr, label_type, at, sms, s) ||
-      !operand(&p.w, f.w, z, dtype, w, w_stride, n_classes, nullptr, label_type, at + f.x.bytes, sms, s))
+  const Lay lx = operand(f.x, z, dtype, x, x_stride, n_rows, nullptr, label_type, at, sms, s);
+  const Lay lw = operand(f.w, z, dtype, w, w_stride, n_classes, nullptr, label_type, at + f.x.bytes, sms, s);
+  if (!lx.map(&p.x_k, 128, kMmaDepth) || !lw.map(&p.w_k, f.pair ? f.n_size / 2 : f.n_size, kMmaDepth))
     return fail(HB_DEVICE_FAILED, "tensor map");
   at += f.x.bytes + f.w.bytes;
   p.part = (float2*)at;
   p.at_label = (float*)(at + f.part);
-  p.pairs = z.planes == 3 ? 6 : 1;
   p.planes = z.planes;
   p.all_classes = (int64_t)n_classes;
   p.width = (int)width;
@@ -287,12 +350,12 @@ hb_status hb_linear_xent_forward(int32_t device, const void* x, uint64_t x_strid
   for (uint64_t r0 = 0; r0 < n_rows; r0 += f.chunk) {
     const uint64_t rows = std::min(f.chunk, n_rows - r0);
     p.part_stride = rows;
-    p.jobs[0] = MmaJob{kJobStats, (int)((rows + m - 1) / m), f.n_tiles, f.n_size, (int)((width + 63) / 64), 1, 1,
+    p.jobs[0] = MmaJob{kJobStats, (int)((rows + m - 1) / m), f.n_tiles, f.n_size, (int)width, stages_of(width), 1, 1,
                        (int)r0, (int)rows, 0, (int)n_classes, {}};
     if (hb_status st = mma_launch(p, f.pair, sms, s)) return st;
     with_xent_types(dtype, label_type, [&](auto, auto l) {
       using L = decltype(l);
-      k_xent_join<L><<<(int)((rows + 255) / 256), 256, 0, s>>>(p.part, f.n_tiles, p.at_label, (const L*)labels + r0, rows, n_classes,
+      k_xent_join<L><<<(int)((rows + 31) / 32), 32 * kJoinWarps, 0, s>>>(p.part, f.n_tiles, p.at_label, (const L*)labels + r0, rows, n_classes,
                                                            loss + r0, lse + r0);
     });
   }
@@ -337,8 +400,11 @@ hb_status hb_linear_xent_backward(int32_t device, const float* dloss, uint64_t d
   }
   char* at = (char*)workspace;
   MmaParams p{};
-  if (!operand(&p.x, b.x, z, dtype, x, x_stride, n_rows, labels, label_type, at, sms, s) ||
-      !operand(&p.w, b.w, z, dtype, w, w_stride, n_classes, nullptr, label_type, at + b.x.bytes, sms, s))
+  const Lay lx = operand(b.x, z, dtype, x, x_stride, n_rows, labels, label_type, at, sms, s);
+  const Lay lw = operand(b.w, z, dtype, w, w_stride, n_classes, nullptr, label_type, at + b.x.bytes, sms, s);
+  const int ctas = b.pair ? 2 : 1, k_rows = 64 * kMmaDepth, out_blocks = b.out_n / ctas / 64;
+  if (!lx.map(&p.x_k, 128, kMmaDepth) || !lw.map(&p.w_k, b.grad_n / ctas, kMmaDepth) || !lx.map(&p.x_mn, k_rows, out_blocks) ||
+      !lw.map(&p.w_mn, k_rows, out_blocks))
     return fail(HB_DEVICE_FAILED, "tensor map");
   at += b.x.bytes + b.w.bytes;
   const uint64_t steps = b.chunks * b.pieces;
@@ -346,7 +412,6 @@ hb_status hb_linear_xent_backward(int32_t device, const float* dloss, uint64_t d
   at = g[1] + b.g_bytes;
   float* dx_acc = (float*)at;
   float* dw_acc = (float*)(at + b.dx_bytes);
-  p.pairs = z.planes == 3 ? 6 : 1;
   p.planes = z.planes;
   p.all_classes = (int64_t)n_classes;
   p.width = (int)width;
@@ -361,11 +426,11 @@ hb_status hb_linear_xent_backward(int32_t device, const float* dloss, uint64_t d
   const auto vec = [&](const void* q) { return (int)(aligned(q, 16) && width * e % 16 == 0 && b.out_n * e % 16 == 0); };
   // dx or dw of `rows` rows from `splits` accumulators
   const auto finish = [&](const float* acc, int splits, uint64_t split_rows, uint64_t rows, void* to) {
-    const int grid = grid_for(rows * width, kFinishThreads, sms);
+    const int grid = grid_for(rows * (b.acc_stride / 4), kFinishThreads, sms), wide = aligned(to, 4 * e) && width % 4 == 0;
     if (dtype == HB_F32)
-      k_xent_finish<float><<<grid, kFinishThreads, 0, s>>>(acc, splits, split_rows, rows, width, b.acc_stride, (float*)to);
+      k_xent_finish<float><<<grid, kFinishThreads, 0, s>>>(acc, splits, split_rows, rows, width, b.acc_stride, wide, (float*)to);
     else
-      k_xent_finish<__nv_bfloat16><<<grid, kFinishThreads, 0, s>>>(acc, splits, split_rows, rows, width, b.acc_stride, (__nv_bfloat16*)to);
+      k_xent_finish<__nv_bfloat16><<<grid, kFinishThreads, 0, s>>>(acc, splits, split_rows, rows, width, b.acc_stride, wide, (__nv_bfloat16*)to);
   };
   // Step i is piece i mod pieces of chunk i / pieces. A launch takes dw and
   // dx of one step's G and forms the next step's, whose small tiles fill up
@@ -377,8 +442,8 @@ hb_status hb_linear_xent_backward(int32_t device, const float* dloss, uint64_t d
       job.row0 = (int)r0, job.n_rows = (int)std::min(b.chunk, n_rows - r0);
       job.class0 = (int)v0, job.n_classes = (int)std::min(b.piece, n_classes - v0);
     };
-    const auto g_map = [&](CUtensorMap* map, const MmaJob& job, uint64_t step, int box_rows) {
-      return mma_map(map, g[step & 1], job.n_classes, job.n_rows, z.planes, b.g_stride, b.chunk * b.g_stride, box_rows);
+    const auto g_lay = [&](const MmaJob& job, uint64_t step) {
+      return Lay{g[step & 1], (uint64_t)job.n_rows, b.g_stride, b.chunk * b.g_stride, z.planes, (job.n_classes + 63) / 64};
     };
     MmaJob done{};
     void *dx_to = nullptr, *dw_to = nullptr;
@@ -386,7 +451,8 @@ hb_status hb_linear_xent_backward(int32_t device, const float* dloss, uint64_t d
     const uint64_t c = (i - 1) / b.pieces, q = (i - 1) % b.pieces;  // of the step done, where i > 0
     if (i > 0) {
       sizes(done, i - 1);
-      if (!g_map(&p.g, done, i - 1, 64)) return fail(HB_DEVICE_FAILED, "tensor map");
+      const Lay lg = g_lay(done, i - 1);
+      if (!lg.map(&p.g_k, 128, kMmaDepth) || !lg.map(&p.g_mn, k_rows, 2)) return fail(HB_DEVICE_FAILED, "tensor map");
       dx_to = (char*)dx + (uint64_t)done.row0 * width * e;
       dw_to = (char*)dw + (uint64_t)done.class0 * width * e;
       acc = b.chunks > 1 ? dw_acc + (uint64_t)done.class0 * b.acc_stride : dw_acc;
@@ -394,19 +460,19 @@ hb_status hb_linear_xent_backward(int32_t device, const float* dloss, uint64_t d
       // splits without any add 0
       MmaJob& jw = p.jobs[p.n_jobs++] = done;
       jw.kind = kJobDw, jw.m_tiles = (done.n_classes + m - 1) / m, jw.n_tiles = out_tiles, jw.n_size = b.out_n;
-      jw.k_blocks = (done.n_rows + 63) / 64, jw.splits = b.dw_splits;
+      jw.k_total = done.n_rows, jw.k_blocks = stages_of(done.n_rows), jw.splits = b.dw_splits;
       jw.out = MmaOut{b.dw_acc ? kOutAcc : out_type, c > 0, vec(dw_to), (int)b.dw_rows, (int)b.acc_stride, acc, dw_to};
       MmaJob& jx = p.jobs[p.n_jobs++] = done;
       jx.kind = kJobDx, jx.m_tiles = (done.n_rows + m - 1) / m, jx.n_tiles = out_tiles, jx.n_size = b.out_n;
-      jx.k_blocks = (done.n_classes + 63) / 64, jx.splits = b.dx_splits;
+      jx.k_total = done.n_classes, jx.k_blocks = stages_of(done.n_classes), jx.splits = b.dx_splits;
       jx.out = MmaOut{b.dx_acc ? kOutAcc : out_type, q > 0, vec(dx_to), (int)b.chunk, (int)b.acc_stride, dx_acc, dx_to};
     }
     if (i < steps) {
       MmaJob& jg = p.jobs[p.n_jobs++] = MmaJob{};
       sizes(jg, i);
-      if (!g_map(&p.g_out, jg, i, 32)) return fail(HB_DEVICE_FAILED, "tensor map");
+      if (!g_lay(jg, i).map(&p.g_out, 32, 1)) return fail(HB_DEVICE_FAILED, "tensor map");
       jg.kind = kJobGrad, jg.m_tiles = (jg.n_rows + m - 1) / m, jg.n_tiles = (jg.n_classes + b.grad_n - 1) / b.grad_n;
-      jg.n_size = b.grad_n, jg.k_blocks = (int)((width + 63) / 64), jg.splits = 1, jg.m_fast = 1;
+      jg.n_size = b.grad_n, jg.k_total = (int)width, jg.k_blocks = stages_of(width), jg.splits = 1, jg.m_fast = 1;
     }
     if (hb_status st = mma_launch(p, b.pair, sms, s)) return st;
     if (i > 0 && b.dw_acc && c + 1 == b.chunks) finish(acc, b.dw_splits, b.dw_rows, done.n_classes, dw_to);

@@ -22,12 +22,14 @@ struct MmaOut {
   void* to;
 };
 
-// m_tiles x n_tiles tiles of (128 x CTAs) x n_size, k in steps of 64 shared
-// among `splits` tiles each; m_fast: consecutive tiles go down the rows.
+constexpr int kMmaDepth = 2;  // blocks of 64 of k in a stage
+
+// m_tiles x n_tiles tiles of (128 x CTAs) x n_size, k (k_total of it) in
+// k_blocks stages shared among `splits` tiles each; m_fast: consecutive tiles go down the rows.
 // The job's rows are [row0, row0 + n_rows) of the call's, its classes
 // [class0, class0 + n_classes) of the layer's.
 struct MmaJob {
-  int kind, m_tiles, n_tiles, n_size, k_blocks, splits, m_fast;
+  int kind, m_tiles, n_tiles, n_size, k_total, k_blocks, splits, m_fast;
   int row0, n_rows, class0, n_classes;
   MmaOut out;
 };
@@ -36,10 +38,13 @@ constexpr int kMaxJobs = 3;
 constexpr int kMaxWorkers = 160;
 
 struct MmaParams {
-  CUtensorMap x, w, g, g_out;  // bf16 [planes][rows][columns]; dx and dw read g, grad writes g_out
+  // the operands (bf16), with the boxes of their two uses: k along memory,
+  // and their own rows along memory
+  CUtensorMap x_k, x_mn, w_k, w_mn, g_k, g_mn;
+  CUtensorMap g_out;           // what grad writes (dx and dw read an earlier launch's)
   MmaJob jobs[kMaxJobs];
   int n_jobs;
-  int pairs, planes;           // 1, 1: bf16; 6, 3: f32 in three pieces
+  int planes;                  // 1: bf16; 3: f32 in three pieces
   int width;
   const void* labels;          // of the call's rows, as the next three
   int label_type;
@@ -60,10 +65,11 @@ struct MmaParams {
   }
 };
 
-// A map of bf16 [planes][rows][cols] with boxes of 64 columns; strides in
-// elements, multiples of 8, the address 16-byte aligned.
-bool mma_map(CUtensorMap* map, const void* p, uint64_t cols, uint64_t rows, uint64_t planes, uint64_t row_stride,
-             uint64_t plane_stride, int box_rows);
+// A map of bf16 [planes][rows][64 * blocks] as [planes][blocks][rows][64],
+// with boxes of box_blocks x box_rows x 64; strides in elements, multiples
+// of 8, the address 16-byte aligned.
+bool mma_map(CUtensorMap* map, const void* p, uint64_t blocks, uint64_t rows, uint64_t planes, uint64_t row_stride,
+             uint64_t plane_stride, int box_rows, int box_blocks);
 // Runs the jobs by single CTAs or (pair) by pairs of them; shares the tiles out.
 hb_status mma_launch(MmaParams& p, bool pair, int sms, cudaStream_t s);
 

@@ -10,10 +10,15 @@
 // CTA t mod grid. A CTA's warp 0 feeds 64-deep steps of both operands
 // through a ring of shared-memory stages by TMA, warp 1 issues the MMAs of a
 // 128 x n tile (n <= 256) into one of two TMEM accumulators, and warps 4 to 7
-// work the other one off. An operand tile is a stack of 64 x 64 blocks
-// whether k or its rows run along memory (tile_desc), so G is written once,
-// row by row, and read as it is by dx (k along memory) and by dw (its
-// classes along memory), and x and w are read as they lie as well.
+// work the other one off. Operands are read as they lie, whether k or their
+// own rows run along memory, so G is written once, row by row, and read by dx
+// (k along memory) and by dw (its classes along memory).
+//
+// Every operand is seen as [plane][block of 64 columns][row][64 columns], so
+// that one copy brings a CTA's whole share of an operand for a stage: with
+// 64 x 64 copies (8 KiB each) the copies themselves were the limit, 990
+// TFLOP/s on 8,192 x 1,024 x 50,021 against 1,330 with 128 x 64 ones. It takes
+// rows of whole blocks: columns past an operand's width are zeros.
 //
 // f32 operands are three bf16 pieces (v = p0 + p1 + p2, each the rounding of
 // what the ones before leave), and a product is the six products of pieces
@@ -32,15 +37,17 @@ namespace {
 
 using namespace hb::mma;
 
-constexpr uint32_t kBlock = 8192;  // bytes of a 64 x 64 block
-constexpr int kThreads = 256;
-// A stage holds 128 rows of A and the CTA's share of up to 256 of B.
+constexpr int kThreads = 384;  // copies, MMAs, two idle warps, 8 warps of the epilogue
+constexpr uint32_t kRow = 128;  // bytes of 64 columns
+// A stage holds kDepth blocks of 64 of k: 128 rows of A and the CTA's share
+// of up to 256 of B.
 template <bool kPair>
 struct Shape {
   static constexpr int kCtas = kPair ? 2 : 1;
-  static constexpr int kStages = kPair ? 6 : 4;
-  static constexpr uint32_t kStageBytes = (kPair ? 4 : 6) * kBlock;
-  static constexpr uint32_t kSmemBytes = 1024 + kStages * kStageBytes + 4 * 2 * 4096 + 256;
+  static constexpr uint32_t kABytes = 128 * kRow * kMmaDepth;
+  static constexpr uint32_t kStageBytes = kABytes + 256 / kCtas * kRow * kMmaDepth;
+  static constexpr int kStages = 196608 / kStageBytes;
+  static constexpr uint32_t kSmemBytes = 1024 + kStages * kStageBytes + 8 * 4096 + 256;
 };
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -54,10 +61,11 @@ __constant__ int kPairB[6] = {0, 2, 1, 0, 1, 0};
 // same for every row (a mean) then does not round each element of a bf16 G
 // the same way, which would not average out: with random factors the
 // gradients are 1.41 of one rounding off, with 1 / n up to 2.4.
+template <bool kSplit>
 __device__ __forceinline__ float unit_of(const MmaParams& p) {
   const uint32_t bits = __float_as_uint(p.dloss[0]);
   const uint32_t e = bits >> 23 & 0xffu;
-  return p.planes > 1 || e == 0u || e == 0xffu ? 1.0f : __uint_as_float((bits & 0x7fffffu) | 0x3f800000u);
+  return kSplit || e == 0u || e == 0xffu ? 1.0f : __uint_as_float((bits & 0x7fffffu) | 0x3f800000u);
 }
 
 template <int kStages>
@@ -70,7 +78,7 @@ struct Ring {
 };
 
 struct TileAt {
-  int m, n, k0, k1, split;
+  int m, n, k0, k1, split;  // k in stages
 };
 
 __device__ __forceinline__ TileAt tile_at(const MmaJob& job, int t) {
@@ -111,14 +119,15 @@ __device__ __forceinline__ void store32(T* dst, const float (&v)[32], int n, boo
   }
 }
 
-template <bool kPair>
+// kSplit: f32 operands in three pieces.
+template <bool kPair, bool kSplit>
 __global__ void __launch_bounds__(kThreads, 1) k_xent_mma(const __grid_constant__ MmaParams p) {
   using S = Shape<kPair>;
   constexpr int kStages = S::kStages;
   extern __shared__ unsigned char raw[];
   const uint32_t base = (smem_addr(raw) + 1023u) & ~1023u;
   const uint32_t staging = base + kStages * S::kStageBytes;
-  const uint32_t bars = staging + 4 * 2 * 4096;
+  const uint32_t bars = staging + 8 * 4096;
   // full: copies landed (a pair's in its first CTA); empty: the MMAs have
   // read a stage; acc_full, acc_empty: the same of an accumulator
   const auto full = [&](int s) { return bars + 8u * s; };
@@ -127,14 +136,15 @@ __global__ void __launch_bounds__(kThreads, 1) k_xent_mma(const __grid_constant_
   const auto acc_empty = [&](int b) { return bars + 8u * (2 * kStages + 2 + b); };
   __shared__ uint32_t s_tmem;
   __shared__ volatile uint32_t s_gave_up;
+  constexpr int kPairs = kSplit ? 6 : 1;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = kPair ? blockIdx.x & 1 : 0, worker = blockIdx.x / S::kCtas;
   if (threadIdx.x == 0) {
     s_gave_up = 0u;
     for (int s = 0; s < kStages; ++s) bar_init(full(s), 1), bar_init(empty(s), 1);
-    for (int b = 0; b < 2; ++b) bar_init(acc_full(b), 1), bar_init(acc_empty(b), 4 * S::kCtas);
+    for (int b = 0; b < 2; ++b) bar_init(acc_full(b), 1), bar_init(acc_empty(b), 8 * S::kCtas);
     bar_init_fence();
-    tma_prefetch(&p.x), tma_prefetch(&p.w);
+    tma_prefetch(&p.x_k), tma_prefetch(&p.w_k);
   }
   if (warp == 2) tmem_alloc<kPair>(smem_addr(&s_tmem), 512);
   fence_before();
@@ -147,31 +157,29 @@ __global__ void __launch_bounds__(kThreads, 1) k_xent_mma(const __grid_constant_
     uint32_t issued = 0;  // stages with a copy in flight or landed
     bool ok = true;
     each_tile(p, worker, [&](const MmaJob& job, const TileAt& at) {
-      const int share = job.n_size / S::kCtas, nb = (share + 63) / 64;  // this CTA's rows of B, and their blocks
-      const CUtensorMap* ma = job.kind == kJobDx || job.kind == kJobDw ? &p.g : &p.x;
-      const CUtensorMap* mb = job.kind == kJobDw ? &p.x : &p.w;
+      const int share = job.n_size / S::kCtas;  // this CTA's rows of B
       const bool a_mn = job.kind == kJobDw, b_mn = job.kind == kJobDx || job.kind == kJobDw;
+      const CUtensorMap* ma = job.kind == kJobDw ? &p.g_mn : job.kind == kJobDx ? &p.g_k : &p.x_k;
+      const CUtensorMap* mb = job.kind == kJobDw ? &p.x_mn : job.kind == kJobDx ? &p.w_mn : &p.w_k;
+      const uint32_t bytes = S::kABytes + share * kRow * kMmaDepth;
       // rows of the operands in their tensors: x starts at the job's first
       // row and w at its first class where those are its rows or its k
-      const int a_row = (at.m * S::kCtas + rank) * 128 + (ma == &p.x ? job.row0 : 0);
-      const int b_row = at.n * job.n_size + rank * share + (mb == &p.w && !b_mn ? job.class0 : 0);
-      const int bk0 = mb == &p.w && b_mn ? job.class0 : mb == &p.x ? job.row0 : 0;
-      for (int q = 6 - p.pairs; q < 6; ++q) {
+      const int a_row = (at.m * S::kCtas + rank) * 128 + (ma == &p.x_k ? job.row0 : 0);
+      const int b_row = at.n * job.n_size + rank * share + (mb == &p.w_k ? job.class0 : 0);
+      const int bk0 = mb == &p.w_mn ? job.class0 : mb == &p.x_mn ? job.row0 : 0;
+      for (int q = 6 - kPairs; q < 6; ++q) {
         const int pa = kPairA[q], pb = kPairB[q];
         for (int k = at.k0; k < at.k1; ++k) {
           if (!(ok = bar_wait(empty(r.stage), r.parity ^ 1u, &s_gave_up))) return false;
           const uint32_t dst = base + r.stage * S::kStageBytes;
           const uint32_t bar = kPair ? peer_addr(full(r.stage), 0) : full(r.stage);
-          if (rank == 0) bar_expect(full(r.stage), (2 + nb) * kBlock * S::kCtas);
+          if (rank == 0) bar_expect(full(r.stage), bytes * S::kCtas);
           issued |= 1u << r.stage;
-          for (int b = 0; b < 2; ++b) {
-            if (a_mn) tma_load<kPair>(dst + b * kBlock, ma, bar, a_row + 64 * b, k * 64, pa);
-            else tma_load<kPair>(dst + b * kBlock, ma, bar, k * 64, a_row + 64 * b, pa);
-          }
-          for (int b = 0; b < nb; ++b) {
-            if (b_mn) tma_load<kPair>(dst + (2 + b) * kBlock, mb, bar, b_row + 64 * b, bk0 + k * 64, pb);
-            else tma_load<kPair>(dst + (2 + b) * kBlock, mb, bar, k * 64, b_row + 64 * b, pb);
-          }
+          // coordinates: column in the block, row, block, plane
+          if (a_mn) tma_load<kPair>(dst, ma, bar, 0, k * 64 * kMmaDepth, a_row >> 6, pa);
+          else tma_load<kPair>(dst, ma, bar, 0, a_row, k * kMmaDepth, pa);
+          if (b_mn) tma_load<kPair>(dst + S::kABytes, mb, bar, 0, bk0 + k * 64 * kMmaDepth, b_row >> 6, pb);
+          else tma_load<kPair>(dst + S::kABytes, mb, bar, 0, b_row, k * kMmaDepth, pb);
           r.next();
         }
       }
@@ -198,146 +206,176 @@ __global__ void __launch_bounds__(kThreads, 1) k_xent_mma(const __grid_constant_
       fence_after();
       const uint32_t d = tmem + buf * 256;
       bool add = false;
-      for (int i = p.pairs * (at.k1 - at.k0); i > 0; --i) {
-        if (!bar_wait(full(r.stage), r.parity, &s_gave_up)) return false;
-        fence_after();
-        const uint32_t dst = base + r.stage * S::kStageBytes;
-        const uint64_t da = tile_desc(dst, a_mn), db = tile_desc(dst + 2 * kBlock, b_mn);
+      // k-major: 16 of k are 32 bytes on, the next block of 64 one block of
+      // rows on; mn-major: 16 of k are 16 rows of 128 bytes on
+      const uint32_t share = job.n_size / S::kCtas;
+      const uint32_t block_a = a_mn ? 64 * kRow >> 4 : 128 * kRow >> 4, block_b = b_mn ? 64 * kRow >> 4 : share * kRow >> 4;
+      for (int q = 0; q < kPairs; ++q)
+        for (int k = at.k0; k < at.k1; ++k) {
+          if (!bar_wait(full(r.stage), r.parity, &s_gave_up)) return false;
+          fence_after();
+          const uint32_t dst = base + r.stage * S::kStageBytes;
+          const uint64_t da = tile_desc(dst, a_mn, 64 * kMmaDepth), db = tile_desc(dst + S::kABytes, b_mn, 64 * kMmaDepth);
+          const int left = job.k_total - k * 64 * kMmaDepth;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          mma_f16<kPair>(d, da + k * sa, db + k * sb, idesc, add);
-          add = true;
+          for (int i = 0; i < 4 * kMmaDepth; ++i) {
+            if (16 * i >= left) break;
+            mma_f16<kPair>(d, da + (i >> 2) * block_a + (i & 3) * sa, db + (i >> 2) * block_b + (i & 3) * sb, idesc, add);
+            add = true;
+          }
+          mma_commit<kPair>(empty(r.stage));
+          r.next();
         }
-        mma_commit<kPair>(empty(r.stage));
-        r.next();
-      }
       mma_commit<kPair>(acc_full(buf));
       ++tile;
       return true;
     });
   } else if (warp >= 4) {
-    const int w4 = warp - 4;
-    const uint32_t stage = staging + w4 * 8192;
-    int tile = 0, stored = 0;
+    // Two warps for each 32 rows, one for each half of the columns: with one,
+    // its waits for TMEM, for exp2 and for its own sums leave the SM idle
+    // while a short k's next tile is ready.
+    const int quarter = warp & 3, half = (warp - 4) >> 2;
+    const uint32_t stage = staging + (warp - 4) * 4096;
+    int tile = 0;
     each_tile(p, worker, [&](const MmaJob& job, const TileAt& at) {
       const int buf = tile & 1;
       const bool ok = bar_wait(acc_full(buf), (tile >> 1) & 1, &s_gave_up);
       __syncwarp();
       fence_after();
-      const uint32_t acc = tmem + buf * 256 + ((uint32_t)(w4 * 32) << 16);
-      const int row0 = (at.m * S::kCtas + rank) * 128 + w4 * 32, row = row0 + lane;
+      const uint32_t acc = tmem + buf * 256 + ((uint32_t)(quarter * 32) << 16);
+      const int row0 = (at.m * S::kCtas + rank) * 128 + quarter * 32, row = row0 + lane;
       const int col0 = at.n * job.n_size;
-      if (job.kind == kJobStats || job.kind == kJobGrad) {
+      const int cut = (job.n_size / 2 + 63) & ~63, c0 = half ? cut : 0, c1 = half ? job.n_size : cut;
+      if (job.kind == kJobStats) {
+        const bool in = row < job.n_rows;
+        const int64_t rel = (in ? p.label((int64_t)job.row0 + row) : -1) - job.class0 - col0;
+        float m = -INFINITY, s = 0.0f;
+        for (int c = c0; c < c1; c += 32) {
+          const int left = job.n_classes - (col0 + c);
+          if (left <= 0) break;
+          float v[32];
+          tmem_load32(acc + c, v);
+          if (left < 32) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] = i < left ? v[i] : -INFINITY;
+          }
+          if (rel >= c && rel < c + 32) {
+            const int hit = (int)rel - c;
+            float z = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 32; ++i) z = hit == i ? v[i] : z;
+            p.at_label[row] = z;
+          }
+          float t[4] = {m, v[0], v[1], v[2]};
+#pragma unroll
+          for (int i = 3; i < 32; ++i) t[i & 3] = fmaxf(t[i & 3], v[i]);
+          const float top = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
+          const float ref = top == -INFINITY ? 0.0f : top * kLog2e;
+          float add[4] = {s * exp2_fast(fmaf(m, kLog2e, -ref)), 0.0f, 0.0f, 0.0f};
+#pragma unroll
+          for (int i = 0; i < 32; ++i) add[i & 3] += exp2_fast(fmaf(v[i], kLog2e, -ref));
+          s = (add[0] + add[1]) + (add[2] + add[3]);
+          m = top;
+        }
+        // the halves meet in the second warp's staging, which no stats tile uses
+        const uint32_t meet = staging + (4 + quarter) * 4096 + buf * 256 + lane * 8;
+        if (half) asm volatile("st.shared.v2.f32 [%0], {%1, %2};" ::"r"(meet), "f"(m), "f"(s) : "memory");
+        asm volatile("bar.sync %0, 64;" ::"r"(quarter + 1) : "memory");
+        if (!half && in) {
+          float2 o;
+          asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(o.x), "=f"(o.y) : "r"(meet) : "memory");
+          const float top = fmaxf(m, o.x), ref = top == -INFINITY ? 0.0f : top * kLog2e;
+          s = s * exp2_fast(fmaf(m, kLog2e, -ref)) + o.y * exp2_fast(fmaf(o.x, kLog2e, -ref));
+          p.part[(size_t)at.n * p.part_stride + row] = ok ? make_float2(top, s) : make_float2(NAN, NAN);
+        }
+      } else if (job.kind == kJobGrad) {
         const bool in = row < job.n_rows;
         const int64_t label = in ? p.label((int64_t)job.row0 + row) : -1;
         const int64_t rel = label - job.class0 - col0;
-        if (job.kind == kJobStats) {
-          float m = -INFINITY, s = 0.0f;
-          for (int c = 0; c < job.n_size; c += 32) {
-            float v[32];
-            tmem_load32(acc + c, v);
-            if (!ok) {
+        // a row without a label: logits and lse 0 (its operand row is 0), factor 0
+        const float each = !ok ? NAN : label >= 0 ? p.dloss[(size_t)(job.row0 + row) * p.dloss_stride] / unit_of<kSplit>(p) : 0.0f;
+        // lse log2(e) as a rounded value and, for f32, what the rounding left
+        const float l = label >= 0 ? p.lse[job.row0 + row] : 0.0f;
+        const float hi = l * kLog2e, lo = kSplit ? fmaf(l, kLog2e, -hi) : 0.0f;
+        for (int c = c0; c < c1; c += 64) {
+          const int left = job.n_classes - (col0 + c);
+          if (left <= 0) break;  // nothing of G there
+          float v[64];
+          tmem_load32(acc + c, reinterpret_cast<float(&)[32]>(v[0]));
+          tmem_load32(acc + c + 32, reinterpret_cast<float(&)[32]>(v[32]));
 #pragma unroll
-              for (int i = 0; i < 32; ++i) v[i] = NAN;
-            }
-            const int left = job.n_classes - (col0 + c);
-            if (left <= 0) break;
-            if (left < 32) {
-#pragma unroll
-              for (int i = 0; i < 32; ++i) v[i] = i < left ? v[i] : -INFINITY;
-            }
-            if (rel >= c && rel < c + 32) {
-              float z = 0.0f;
-#pragma unroll
-              for (int i = 0; i < 32; ++i) z = rel == c + i ? v[i] : z;
-              p.at_label[row] = z;
-            }
-            float top = m;
-#pragma unroll
-            for (int i = 0; i < 32; ++i) top = fmaxf(top, v[i]);
-            const float ref = top == -INFINITY ? 0.0f : top * kLog2e;
-            float add = 0.0f;
-#pragma unroll
-            for (int i = 0; i < 32; ++i) add += exp2_fast(fmaf(v[i], kLog2e, -ref));
-            s = fmaf(s, exp2_fast(fmaf(m, kLog2e, -ref)), add);
-            m = top;
+          for (int i = 0; i < 64; ++i) {
+            float g = fmaf(v[i], kLog2e, -hi);
+            if (kSplit) g -= lo;
+            v[i] = exp2_fast(g);
           }
-          if (in) p.part[(size_t)at.n * p.part_stride + row] = make_float2(m, s);
-        } else {
-          const float each = label >= 0 ? p.dloss[(size_t)(job.row0 + row) * p.dloss_stride] / unit_of(p) : 0.0f;
-          // lse log2(e) as a rounded value and what the rounding left
-          const float l = in ? p.lse[job.row0 + row] : 0.0f;
-          const float hi = l * kLog2e, lo = fmaf(l, kLog2e, -hi);
-          for (int c = 0; c < job.n_size; c += 64) {
-            float v[64];
-            tmem_load32(acc + c, reinterpret_cast<float(&)[32]>(v[0]));
-            tmem_load32(acc + c + 32, reinterpret_cast<float(&)[32]>(v[32]));
+          if (rel >= c && rel < c + 64) {
+            const int hit = (int)rel - c;
 #pragma unroll
-            for (int i = 0; i < 64; ++i) {
-              float g = exp2_fast(fmaf(v[i], kLog2e, -hi) - lo);
-              if (rel == c + i) g -= 1.0f;
-              v[i] = label < 0 ? 0.0f : ok ? each * g : NAN;
-            }
-            if (col0 + c >= job.n_classes) break;  // nothing of G there
-            for (int q = 0; q < p.planes; ++q) {
-              const uint32_t out = stage + (stored & 1) * 4096;
-              if (lane == 0) tma_wait_read<1>();
-              __syncwarp();
+            for (int i = 0; i < 64; ++i) v[i] -= hit == i ? 1.0f : 0.0f;
+          }
 #pragma unroll
-              for (int i = 0; i < 8; ++i) {
-                uint32_t h[4];
+          for (int i = 0; i < 64; ++i) v[i] *= each;
+          if (left < 64) {  // zeros up to the block's end: dx reads it whole
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                  const __nv_bfloat162 b = __floats2bfloat162_rn(v[8 * i + 2 * j], v[8 * i + 2 * j + 1]);
-                  h[j] = *reinterpret_cast<const uint32_t*>(&b);
-                  if (p.planes > 1) {
-                    v[8 * i + 2 * j] -= __low2float(b);
-                    v[8 * i + 2 * j + 1] -= __high2float(b);
-                  }
+            for (int i = 0; i < 64; ++i) v[i] = i < left ? v[i] : 0.0f;
+          }
+#pragma unroll
+          for (int q = 0; q < (kSplit ? 3 : 1); ++q) {
+            if (lane == 0) tma_wait_read<0>();
+            __syncwarp();
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              uint32_t h[4];
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                const __nv_bfloat162 b = __floats2bfloat162_rn(v[8 * i + 2 * j], v[8 * i + 2 * j + 1]);
+                h[j] = *reinterpret_cast<const uint32_t*>(&b);
+                if (kSplit) {
+                  v[8 * i + 2 * j] -= __low2float(b);
+                  v[8 * i + 2 * j + 1] -= __high2float(b);
                 }
-                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(out + lane * 128 + ((i ^ (lane & 7)) << 4)), "r"(h[0]),
-                             "r"(h[1]), "r"(h[2]), "r"(h[3])
-                             : "memory");
               }
-              proxy_fence();
-              __syncwarp();
-              if (lane == 0 && row0 < job.n_rows) {
-                tma_store(&p.g_out, out, col0 + c, row0, q);
-                tma_commit();
-              }
-              ++stored;
+              asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(stage + lane * 128 + ((i ^ (lane & 7)) << 4)), "r"(h[0]),
+                           "r"(h[1]), "r"(h[2]), "r"(h[3])
+                           : "memory");
+            }
+            proxy_fence();
+            __syncwarp();
+            if (lane == 0 && row0 < job.n_rows) {
+              tma_store(&p.g_out, stage, 0, row0, (col0 + c) >> 6, q);
+              tma_commit();
             }
           }
         }
       } else {
         const int rows = job.kind == kJobDx ? job.n_rows : job.n_classes;
         const MmaOut& o = job.out;
-        const float unit = unit_of(p);
-        for (int c = 0; c < job.n_size; c += 32) {
-          float v[32];
-          tmem_load32(acc + c, v);
-          if (!ok || at.k0 == at.k1) {  // no step of k fell to this split
-#pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] = ok ? 0.0f : NAN;
-          }
+        // no step of k fell to an empty split: its accumulator is not written
+        const float unit = !ok ? NAN : unit_of<kSplit>(p);
+        const bool none = at.k0 == at.k1;
+        for (int c = c0; c < c1; c += 32) {
           const int left = p.width - (col0 + c);
           if (left <= 0) break;
+          float v[32];
+          tmem_load32(acc + c, v);
 #pragma unroll
-          for (int i = 0; i < 32; ++i) v[i] *= unit;
+          for (int i = 0; i < 32; ++i) v[i] = none ? 0.0f : v[i] * unit;
           if (row < rows) {
             const int n = left < 32 ? left : 32;
             if (o.type == kOutAcc) {
-              // accumulators' rows are padded to whole groups of four
-              float4* q = reinterpret_cast<float4*>(o.acc + ((size_t)at.split * o.split_rows + row) * o.acc_stride + col0 + c);
+              // accumulators' rows are padded to whole groups of four; each
+              // element is added to once a launch, so the order is the launches'
+              float* q = o.acc + ((size_t)at.split * o.split_rows + row) * o.acc_stride + col0 + c;
 #pragma unroll
               for (int i = 0; i < 8; ++i)
                 if (4 * i < n) {
-                  float4 u = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
-                  if (o.add) {
-                    const float4 b = q[i];
-                    u.x += b.x, u.y += b.y, u.z += b.z, u.w += b.w;
-                  }
-                  q[i] = u;
+                  if (o.add)
+                    asm volatile("red.relaxed.gpu.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(q + 4 * i), "f"(v[4 * i]),
+                                 "f"(v[4 * i + 1]), "f"(v[4 * i + 2]), "f"(v[4 * i + 3])
+                                 : "memory");
+                  else
+                    *reinterpret_cast<float4*>(q + 4 * i) = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
                 }
             } else if (o.type == kOutF32) {
               store32((float*)o.to + (size_t)row * p.width + col0 + c, v, n, o.vec);
@@ -383,28 +421,28 @@ EncodeFn encoder() {
 
 }  // namespace
 
-bool mma_map(CUtensorMap* map, const void* p, uint64_t cols, uint64_t rows, uint64_t planes, uint64_t row_stride,
-             uint64_t plane_stride, int box_rows) {
+bool mma_map(CUtensorMap* map, const void* p, uint64_t blocks, uint64_t rows, uint64_t planes, uint64_t row_stride,
+             uint64_t plane_stride, int box_rows, int box_blocks) {
   const EncodeFn fn = encoder();
   if (!fn) return false;
-  const cuuint64_t dims[3] = {cols, rows, planes};
-  const cuuint64_t strides[2] = {2 * row_stride, 2 * plane_stride};
-  const cuuint32_t box[3] = {64, (cuuint32_t)box_rows, 1}, step[3] = {1, 1, 1};
-  return fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(p), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+  const cuuint64_t dims[4] = {64, rows, blocks, planes};
+  const cuuint64_t strides[3] = {2 * row_stride, 128, 2 * plane_stride};
+  const cuuint32_t box[4] = {64, (cuuint32_t)box_rows, (cuuint32_t)box_blocks, 1}, step[4] = {1, 1, 1, 1};
+  return fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(p), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 namespace {
 
 // Shares the jobs' tiles out among the workers in the jobs' order: each
-// job's tiles go where the least work is so far (a tile's work: its steps of
-// k and about three more), as far as whole tiles allow.
+// job's tiles go where the least work is so far (a tile's work: its blocks
+// of k and about three more), as far as whole tiles allow.
 void share_out(MmaParams& p, int workers) {
   long long load[kMaxWorkers] = {};
   for (int j = 0; j < p.n_jobs; ++j) {
     const MmaJob& job = p.jobs[j];
     const long long tiles = (long long)job.m_tiles * job.n_tiles * job.splits;
-    const long long cost = (long long)p.pairs * job.k_blocks / job.splits + 3;
+    const long long cost = (p.planes > 1 ? 6ll : 1ll) * kMmaDepth * job.k_blocks / job.splits + 3;
     const auto below = [&](long long level) {
       long long n = 0;
       for (int u = 0; u < workers; ++u) n += level > load[u] ? (level - load[u]) / cost : 0;
@@ -430,14 +468,14 @@ void share_out(MmaParams& p, int workers) {
   }
 }
 
-template <bool kPair>
+template <bool kPair, bool kSplit>
 hb_status launch(const MmaParams& p, int workers, cudaStream_t s) {
   using S = Shape<kPair>;
   static thread_local int ready = -1;
   int device = 0;
   cudaGetDevice(&device);
   if (ready != device) {
-    if (cudaFuncSetAttribute(k_xent_mma<kPair>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmemBytes) != cudaSuccess)
+    if (cudaFuncSetAttribute(k_xent_mma<kPair, kSplit>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmemBytes) != cudaSuccess)
       return fail(HB_DEVICE_FAILED, "shared memory of the product kernel");
     ready = device;
   }
@@ -451,7 +489,7 @@ hb_status launch(const MmaParams& p, int workers, cudaStream_t s) {
   a[0].val.clusterDim = {S::kCtas, 1, 1};
   c.attrs = a;
   c.numAttrs = kPair ? 1 : 0;
-  const cudaError_t e = cudaLaunchKernelEx(&c, k_xent_mma<kPair>, p);
+  const cudaError_t e = cudaLaunchKernelEx(&c, k_xent_mma<kPair, kSplit>, p);
   if (e == cudaSuccess) return HB_OK;
   cudaGetLastError();
   return fail(HB_DEVICE_FAILED, std::string("product kernel: ") + cudaGetErrorString(e));
@@ -466,7 +504,8 @@ hb_status mma_launch(MmaParams& p, bool pair, int sms, cudaStream_t s) {
   const int most = std::min(pair ? sms / 2 : sms, kMaxWorkers);
   const int workers = (int)std::min<long long>(tiles, std::max(most, 1));
   share_out(p, workers);
-  return pair ? launch<true>(p, workers, s) : launch<false>(p, workers, s);
+  if (p.planes > 1) return pair ? launch<true, true>(p, workers, s) : launch<false, true>(p, workers, s);
+  return pair ? launch<true, false>(p, workers, s) : launch<false, false>(p, workers, s);
 }
 
 }  // namespace head
