@@ -65,9 +65,9 @@ __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2hal
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
-// V elements of T moved by one load or store.
+// V elements of T moved by one 16-byte load or store, or by two.
 template <typename T, int V>
-struct alignas(sizeof(T) * V) Pack {
+struct alignas(sizeof(T) * V < 16 ? sizeof(T) * V : 16) Pack {
   T v[V];
 };
 
