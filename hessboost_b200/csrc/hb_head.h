@@ -9,6 +9,7 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <cstdint>
 #include <string>
 
@@ -70,6 +71,19 @@ template <typename T, int V>
 struct alignas(sizeof(T) * V < 16 ? sizeof(T) * V : 16) Pack {
   T v[V];
 };
+
+// Lets kernel K have `bytes` of dynamic shared memory on the device (as much
+// as there may be, once a device).
+template <auto K>
+void allow_shared(int device, uint32_t bytes) {
+  static std::atomic<uint64_t> done{0};
+  const uint64_t bit = 1ull << (device & 63);
+  if (bytes <= 32 * 1024 || (done.load(std::memory_order_relaxed) & bit)) return;
+  cudaFuncAttributes a;
+  if (cudaFuncGetAttributes(&a, K) != cudaSuccess) return;
+  if (cudaFuncSetAttribute(K, cudaFuncAttributeMaxDynamicSharedMemorySize, 232448 - (int)a.sharedSizeBytes) == cudaSuccess && device < 64)
+    done.fetch_or(bit, std::memory_order_relaxed);
+}
 
 // Calls f with a value of the element type `dtype` names (checked before).
 template <typename F>

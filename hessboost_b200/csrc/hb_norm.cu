@@ -657,10 +657,6 @@ hb_status check_norm(int32_t dtype, int32_t param, uint64_t n_rows, uint32_t wid
 uint64_t resident(int threads, uint32_t bytes, int regs) {
   return (uint64_t)std::max(1, std::min({1536 / threads, (int)(220000 / (bytes + 9000)), 65536 / (threads * regs)}));
 }
-// Lets the kernel have `bytes` of dynamic shared memory.
-void allow_shared(const void* kernel, uint32_t bytes) {
-  if (bytes > 32 * 1024) cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
-}
 // Rows of partial sums of a backward call.
 uint64_t norm_parts(uint64_t n_rows) { return std::max<uint64_t>(1, std::min(n_rows, kParts)); }
 
@@ -708,7 +704,7 @@ hb_status hb_layer_norm_forward(int32_t device, const void* x, int32_t dtype, ui
       const int threads = kBlock ? p.size : kGroupThreads;
       const uint32_t bytes = RowRing<T, V, N, 1, kRingStages<kBlock>, kBlock>::bytes(threads, kBlock ? 32 : p.size);
       const uint64_t grid = std::min<uint64_t>((n_rows + rows - 1) / rows, resident(threads, bytes, N * V * 3 + 30) * sms);
-      allow_shared((const void*)k_norm_forward<T, P, V, N, kBlock>, bytes);
+      allow_shared<k_norm_forward<T, P, V, N, kBlock>>(device, bytes);
       k_norm_forward<T, P, V, N, kBlock><<<(unsigned)grid, threads, bytes, s>>>(
           (const T*)x, x_stride, n_rows, width, p.size, (const P*)weight, (const P*)bias, eps, (T*)y, mean, rstd);
     });
@@ -777,7 +773,7 @@ hb_status hb_layer_norm_backward(int32_t device, const void* dy, uint64_t dy_str
         const uint32_t bytes = kBlock ? ring : std::max<uint32_t>(ring, 8 * (kGroupThreads / 32) * width);
         const uint64_t most = std::min<uint64_t>(kParts, resident(threads, bytes, N * V * 5 + 35) * sms);
         grid = std::min<uint64_t>((n_rows + rows - 1) / rows, most);
-        allow_shared((const void*)k_norm_backward<T, P, V, N, kBlock>, bytes);
+        allow_shared<k_norm_backward<T, P, V, N, kBlock>>(device, bytes);
         k_norm_backward<T, P, V, N, kBlock><<<(unsigned)grid, threads, bytes, s>>>(
             (const T*)dy, dy_stride, (const T*)x, x_stride, n_rows, width, p.size, (const P*)weight, mean, rstd, (T*)dx, part,
             (P*)dweight, (P*)dbias);
