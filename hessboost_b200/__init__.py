@@ -301,7 +301,7 @@ SIGNATURES = {
     "hb_linear_xent_backward_workspace": [_i32, _vp, _u64, _vp, _u64, _i32, _u64, _u32, _u64, _u64p],
     "hb_linear_xent_backward": [_i32, _vp, _u64, _vp, _u64, _vp, _u64, _i32, _vp, _i32, _vp, _u64, _u32, _u64,
         _vp, _vp, _vp, _u64, _vp],
-    "hb_grad_norm_workspace": [_i32, _vp, _u64p],
+    "hb_grad_norm_workspace": [_i32, _i32, _u64p],
     "hb_grad_norm": [_i32, _i32, _vp, _vp, _vp, _vp, _vp, _u64, _vp],
     "hb_clip_grad_norm": [_i32, _i32, _vp, _vp, _vp, _vp, _f32, _vp, _vp, _u64, _vp],
 }

@@ -4,6 +4,15 @@
 //   out  = g * min(1, max_norm / (norm + 1e-6))
 //
 // A norm that is not finite passes into every output through the factor.
+// Squares and the sums of a chunk (up to 32 squares a thread) are f32, the
+// rest of the sum f64, in an order that the sizes alone decide.
+//
+// Bound by memory: everything is read, and for clipping read again and
+// written. Tensors are cut into chunks of 1,024 vectors of 16 bytes, and each
+// CTA takes a run of chunks, whatever the tensors' sizes. The second reading
+// goes through each run backwards: what the first one left in the L2 cache is
+// its end. Clipping has no kernel for the norm between the two: every CTA adds
+// the first kernel's sums itself.
 #include <algorithm>
 
 #include "hb_head.h"
@@ -13,22 +22,26 @@ namespace head {
 namespace {
 
 constexpr int kClipThreads = 256;
-constexpr uint64_t kChunk = 65536;  // elements of one CTA's share of a tensor
-constexpr int kTable = 512;         // tensors of one launch
+constexpr int kEach = 4;                               // vectors a thread of a chunk
+constexpr uint32_t kChunk = kClipThreads * kEach;      // vectors
+constexpr int kSmall = 24, kLarge = 512;               // tensors of a launch
+constexpr int kCtasPerSm = 8;
 
-// The tensors of one launch, passed as a kernel argument (no device copy of
+// The tensors of a launch, passed as a kernel argument (no device copy of
 // the table). first[i] = chunks before tensor i.
+template <int kTable>
 struct Table {
   const void* in[kTable];
   void* out[kTable];
-  uint64_t size[kTable];
+  uint64_t n[kTable];
   uint32_t first[kTable + 1];
   uint8_t dtype[kTable];
-  int n;
+  int count;
 };
 
-__device__ __forceinline__ int tensor_of(const Table& t, uint32_t chunk) {
-  int lo = 0, hi = t.n - 1;  // last tensor whose first chunk is <= chunk
+template <int kTable>
+__device__ __forceinline__ int tensor_of(const Table<kTable>& t, uint32_t chunk) {
+  int lo = 0, hi = t.count - 1;  // last tensor whose first chunk is <= chunk
   while (lo < hi) {
     const int m = (lo + hi + 1) >> 1;
     if (t.first[m] <= chunk) lo = m; else hi = m - 1;
@@ -36,60 +49,174 @@ __device__ __forceinline__ int tensor_of(const Table& t, uint32_t chunk) {
   return lo;
 }
 
+// A tensor's vectors: elements [head, head + V count) on 16-byte boundaries
+// of `at`, of which in[] is `shift` elements past such a boundary. With a
+// shift a vector comes from two units of the input, both wholly inside it.
+// The elements before and after are taken singly.
+struct Span {
+  uint64_t head, count;
+  uint32_t shift;
+};
 template <typename T>
-__device__ float square_sum(const void* p, uint64_t b, uint64_t e) {
-  const T* v = (const T*)p;
-  float acc = 0.0f;
-  for (uint64_t i = b + threadIdx.x; i < e; i += kClipThreads) {
-    const float x = to_f32(v[i]);
-    acc = fmaf(x, x, acc);
-  }
-  return acc;
+__device__ __forceinline__ Span span_of(const T* in, const T* at, uint64_t n) {
+  constexpr uint32_t V = 16 / sizeof(T);
+  Span s;
+  s.head = (16 - (reinterpret_cast<uintptr_t>(at) & 15)) % 16 / sizeof(T);
+  if (s.head >= n) return {n, 0, 0};
+  s.shift = (uint32_t)(reinterpret_cast<uintptr_t>(in + s.head) & 15) / sizeof(T);
+  if (s.shift > s.head) s.head += V;  // the first unit begins before the tensor
+  const uint64_t left = n > s.head ? n - s.head : 0;
+  s.count = s.shift ? (left + s.shift) / V : left / V;
+  if (s.shift) s.count = s.count ? s.count - 1 : 0;
+  return s;
 }
 
-__device__ double block_sum(double v) {
-  __shared__ double s[kClipThreads];
-  s[threadIdx.x] = v;
+// The 16 bytes `shift` bytes into the 32 of a and b (a multiple of 2, below 16).
+__device__ __forceinline__ uint4 shifted(uint4 a, uint4 b, uint32_t shift) {
+  uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+  if (shift & 8) {
+#pragma unroll
+    for (int i = 0; i < 6; ++i) w[i] = w[i + 2];
+  }
+  if (shift & 4) {
+#pragma unroll
+    for (int i = 0; i < 5; ++i) w[i] = w[i + 1];
+  }
+  if (shift & 2) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = __funnelshift_r(w[i], w[i + 1], 16);
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// The block's sum of v, for every thread.
+__device__ __forceinline__ double block_sum(double v) {
+  __shared__ double s[kClipThreads / 32];
+#pragma unroll
+  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = v;
   __syncthreads();
-  for (int o = kClipThreads / 2; o; o >>= 1) {
-    if (threadIdx.x < o) s[threadIdx.x] += s[threadIdx.x + o];
-    __syncthreads();
-  }
-  return s[0];
-}
-
-__global__ void __launch_bounds__(kClipThreads) k_square_sums(const __grid_constant__ Table t, double* __restrict__ sums) {
-  const int i = tensor_of(t, blockIdx.x);
-  const uint64_t b = (uint64_t)(blockIdx.x - t.first[i]) * kChunk, e = min(b + kChunk, t.size[i]);
-  const float v = t.dtype[i] == HB_F32   ? square_sum<float>(t.in[i], b, e)
-                  : t.dtype[i] == HB_F16 ? square_sum<__half>(t.in[i], b, e)
-                                         : square_sum<__nv_bfloat16>(t.in[i], b, e);
-  const double all = block_sum((double)v);
-  if (threadIdx.x == 0) sums[blockIdx.x] = all;
-}
-
-__global__ void __launch_bounds__(kClipThreads) k_norm(const double* __restrict__ sums, uint64_t n, float* __restrict__ norm) {
-  double v = 0.0;
-  for (uint64_t i = threadIdx.x; i < n; i += kClipThreads) v += sums[i];
-  v = block_sum(v);
-  if (threadIdx.x == 0) *norm = (float)sqrt(v);
+  v = s[0];
+#pragma unroll
+  for (int w = 1; w < kClipThreads / 32; ++w) v += s[w];
+  return v;
 }
 
 template <typename T>
-__device__ void scale_chunk(const void* in, void* out, uint64_t b, uint64_t e, float by) {
-  const T* v = (const T*)in;
-  T* o = (T*)out;
-  for (uint64_t i = b + threadIdx.x; i < e; i += kClipThreads) o[i] = from_f32<T>(to_f32(v[i]) * by);
+__device__ __forceinline__ float squares(const T* in, uint64_t n, uint32_t chunk) {
+  constexpr int V = 16 / sizeof(T);
+  const Span s = span_of(in, in, n);
+  float acc[4] = {};
+  Pack<T, V> q[kEach];
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {
+    const uint64_t j = (uint64_t)chunk * kChunk + i * kClipThreads + threadIdx.x;
+    if (j < s.count) q[i] = reinterpret_cast<const Pack<T, V>*>(in + s.head)[j];
+  }
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {
+    const uint64_t j = (uint64_t)chunk * kChunk + i * kClipThreads + threadIdx.x;
+    if (j < s.count) {
+#pragma unroll
+      for (int k = 0; k < V; ++k) {
+        const float x = to_f32(q[i].v[k]);
+        acc[k & 3] = fmaf(x, x, acc[k & 3]);
+      }
+    }
+  }
+  if (chunk == 0) {
+    const uint64_t ends = n - s.count * V;  // single elements: s.head before the vectors, the others after
+    for (uint64_t k = threadIdx.x; k < ends; k += kClipThreads) {
+      const float x = to_f32(in[k < s.head ? k : k + s.count * V]);
+      acc[0] = fmaf(x, x, acc[0]);
+    }
+  }
+  return (acc[0] + acc[1]) + (acc[2] + acc[3]);
 }
 
-__global__ void __launch_bounds__(kClipThreads) k_clip(const __grid_constant__ Table t, const float* __restrict__ norm, float max_norm) {
-  const float q = max_norm / (*norm + 1e-6f);
+template <int kTable>
+__global__ void __launch_bounds__(kClipThreads) k_square_sums(const __grid_constant__ Table<kTable> t, double* __restrict__ sums) {
+  const uint32_t chunks = t.first[t.count];
+  const uint32_t c0 = (uint32_t)((uint64_t)chunks * blockIdx.x / gridDim.x), c1 = (uint32_t)((uint64_t)chunks * (blockIdx.x + 1) / gridDim.x);
+  double v = 0.0;
+  int i = tensor_of(t, c0);
+  for (uint32_t c = c0; c < c1; ++c) {
+    while (c >= t.first[i + 1]) ++i;
+    const uint32_t k = c - t.first[i];
+    v += (double)(t.dtype[i] == HB_F32   ? squares((const float*)t.in[i], t.n[i], k)
+                  : t.dtype[i] == HB_F16 ? squares((const __half*)t.in[i], t.n[i], k)
+                                         : squares((const __nv_bfloat16*)t.in[i], t.n[i], k));
+  }
+  v = block_sum(v);
+  if (threadIdx.x == 0) sums[blockIdx.x] = v;
+}
+
+// The norm from the CTAs' sums, for every thread of the block.
+__device__ __forceinline__ float norm_of(const double* __restrict__ sums, uint32_t n) {
+  double v = 0.0;
+  for (uint32_t i = threadIdx.x; i < n; i += kClipThreads) v += sums[i];
+  return (float)sqrt(block_sum(v));
+}
+
+__global__ void __launch_bounds__(kClipThreads) k_norm(const double* __restrict__ sums, uint32_t n, float* __restrict__ norm) {
+  const float v = norm_of(sums, n);
+  if (threadIdx.x == 0) *norm = v;
+}
+
+template <typename T>
+__device__ __forceinline__ void scale_chunk(const T* in, T* out, uint64_t n, uint32_t chunk, float by) {
+  constexpr int V = 16 / sizeof(T);
+  const Span s = span_of(in, out, n);
+  const uint4* units = reinterpret_cast<const uint4*>(in + s.head - s.shift);
+  uint4 a[kEach], b[kEach];
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {
+    const uint64_t j = (uint64_t)chunk * kChunk + i * kClipThreads + threadIdx.x;
+    if (j < s.count) {
+      a[i] = units[j];
+      if (s.shift) b[i] = units[j + 1];
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {
+    const uint64_t j = (uint64_t)chunk * kChunk + i * kClipThreads + threadIdx.x;
+    if (j < s.count) {
+      uint4 u = s.shift ? shifted(a[i], b[i], s.shift * sizeof(T)) : a[i];
+      Pack<T, V>& q = reinterpret_cast<Pack<T, V>&>(u);
+#pragma unroll
+      for (int k = 0; k < V; ++k) q.v[k] = from_f32<T>(to_f32(q.v[k]) * by);
+      __stcs(reinterpret_cast<uint4*>(out + s.head) + j, u);  // not read again: the cache is for what is
+    }
+  }
+  if (chunk == 0) {
+    const uint64_t ends = n - s.count * V;
+    for (uint64_t k = threadIdx.x; k < ends; k += kClipThreads) {
+      const uint64_t at = k < s.head ? k : k + s.count * V;
+      out[at] = from_f32<T>(to_f32(in[at]) * by);
+    }
+  }
+}
+
+// out = in for a launch's tensors, scaled by the norm of all launches' sums;
+// in and out may be the same tensors.
+template <int kTable>
+__global__ void __launch_bounds__(kClipThreads)
+    k_clip(const __grid_constant__ Table<kTable> t, const double* __restrict__ sums, uint32_t n_sums, float max_norm, float* __restrict__ norm) {
+  const float all = norm_of(sums, n_sums);
+  if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = all;
+  const float q = max_norm / (all + 1e-6f);
   const float by = q > 1.0f ? 1.0f : q;  // NaN stays NaN
-  const int i = tensor_of(t, blockIdx.x);
-  const uint64_t b = (uint64_t)(blockIdx.x - t.first[i]) * kChunk, e = min(b + kChunk, t.size[i]);
-  if (t.dtype[i] == HB_F32) scale_chunk<float>(t.in[i], t.out[i], b, e, by);
-  else if (t.dtype[i] == HB_F16) scale_chunk<__half>(t.in[i], t.out[i], b, e, by);
-  else scale_chunk<__nv_bfloat16>(t.in[i], t.out[i], b, e, by);
+  const uint32_t chunks = t.first[t.count];
+  const uint32_t c0 = (uint32_t)((uint64_t)chunks * blockIdx.x / gridDim.x), c1 = (uint32_t)((uint64_t)chunks * (blockIdx.x + 1) / gridDim.x);
+  if (c0 == c1) return;
+  int i = tensor_of(t, c1 - 1);
+  for (uint32_t c = c1; c-- > c0;) {
+    while (c < t.first[i]) --i;
+    const uint32_t k = c - t.first[i];
+    if (t.dtype[i] == HB_F32) scale_chunk((const float*)t.in[i], (float*)t.out[i], t.n[i], k, by);
+    else if (t.dtype[i] == HB_F16) scale_chunk((const __half*)t.in[i], (__half*)t.out[i], t.n[i], k, by);
+    else scale_chunk((const __nv_bfloat16*)t.in[i], (__nv_bfloat16*)t.out[i], t.n[i], k, by);
+  }
 }
 
 hb_status check_tensors(int32_t n, const void* const* tensors, const uint64_t* sizes, const int32_t* dtypes) {
@@ -97,50 +224,51 @@ hb_status check_tensors(int32_t n, const void* const* tensors, const uint64_t* s
   HB_HEAD_REQUIRE(n == 0 || (tensors && sizes && dtypes), "tensors, sizes or dtypes is NULL");
   for (int i = 0; i < n; ++i) {
     HB_HEAD_REQUIRE(known_type(dtypes[i]), "unknown element type");
-    HB_HEAD_REQUIRE(sizes[i] < (1ull << 46), "a tensor is too large");
+    HB_HEAD_REQUIRE(sizes[i] < (1ull << 42), "a tensor is too large");
     HB_HEAD_REQUIRE(tensors[i] || !sizes[i], "a tensor is NULL");
     HB_HEAD_REQUIRE(aligned(tensors[i], size_of(dtypes[i])), "a tensor is not aligned to its type");
   }
   return HB_OK;
 }
 
-uint64_t chunks_of(int32_t n, const uint64_t* sizes) {
-  uint64_t c = 0;
-  for (int i = 0; i < n; ++i) c += (sizes[i] + kChunk - 1) / kChunk;
-  return c;
+// Chunks of a tensor: of its vectors, one at least for its other elements.
+uint32_t chunks_of(uint64_t n, int32_t dtype) {
+  return (uint32_t)std::max<uint64_t>(1, (n * size_of(dtype) / 16 + kChunk - 1) / kChunk);
 }
+uint32_t ctas_of(uint32_t chunks, int sms) { return std::min(chunks, (uint32_t)(sms * kCtasPerSm)); }
 
-// f(table, chunks, first chunk of the launch) for every group of kTable tensors.
-template <typename F>
-void each_table(int32_t n, const void* const* tensors, void* const* outs, const uint64_t* sizes, const int32_t* dtypes, F&& f) {
-  uint64_t before = 0;
-  Table t;
+// f(table of the next tensors, CTAs) for group after group of them.
+template <int kTable, typename F>
+void each_table(int32_t n, const void* const* tensors, void* const* outs, const uint64_t* sizes, const int32_t* dtypes, int sms, F&& f) {
+  Table<kTable> t;
   for (int a = 0; a < n;) {
-    t.n = 0;
+    t.count = 0;
     uint32_t c = 0;
-    for (; a < n && t.n < kTable && c < (1u << 30); ++a) {
+    for (; a < n && t.count < kTable && c < (1u << 30); ++a) {
       if (!sizes[a]) continue;
-      t.in[t.n] = tensors[a];
-      t.out[t.n] = outs ? outs[a] : nullptr;
-      t.size[t.n] = sizes[a];
-      t.dtype[t.n] = (uint8_t)dtypes[a];
-      t.first[t.n++] = c;
-      c += (uint32_t)((sizes[a] + kChunk - 1) / kChunk);
+      t.in[t.count] = tensors[a];
+      t.out[t.count] = outs ? outs[a] : nullptr;
+      t.n[t.count] = sizes[a];
+      t.dtype[t.count] = (uint8_t)dtypes[a];
+      t.first[t.count++] = c;
+      c += chunks_of(sizes[a], dtypes[a]);
     }
-    if (c) f(t, c, before);
-    before += c;
+    t.first[t.count] = c;
+    if (c) f(t, ctas_of(c, sms));
   }
 }
+// Sums that a call's launches leave, at most: a launch's tensors are full
+// groups but the last's.
+uint64_t most_sums(int32_t n, int sms) { return (uint64_t)(n / kLarge + 2) * sms * kCtasPerSm; }
 
-hb_status norm_launch(int32_t n, const void* const* tensors, const uint64_t* sizes, const int32_t* dtypes,
-                      float* norm, double* sums, cudaStream_t s) {
-  uint64_t total = 0;
-  each_table(n, tensors, nullptr, sizes, dtypes, [&](const Table& t, uint32_t chunks, uint64_t before) {
-    k_square_sums<<<chunks, kClipThreads, 0, s>>>(t, sums + before);
-    total = before + chunks;
+template <int kTable>
+uint32_t sum_launches(int32_t n, const void* const* tensors, const uint64_t* sizes, const int32_t* dtypes, double* sums, int sms, cudaStream_t s) {
+  uint32_t before = 0;
+  each_table<kTable>(n, tensors, nullptr, sizes, dtypes, sms, [&](const Table<kTable>& t, uint32_t ctas) {
+    k_square_sums<kTable><<<ctas, kClipThreads, 0, s>>>(t, sums + before);
+    before += ctas;
   });
-  k_norm<<<1, kClipThreads, 0, s>>>(sums, total, norm);
-  return launched("hb_grad_norm");
+  return before;
 }
 
 }  // namespace
@@ -151,10 +279,10 @@ using namespace hb::head;
 
 extern "C" {
 
-hb_status hb_grad_norm_workspace(int32_t n_tensors, const uint64_t* sizes, uint64_t* bytes) {
+hb_status hb_grad_norm_workspace(int32_t device, int32_t n_tensors, uint64_t* bytes) {
   begin_call();
-  HB_HEAD_REQUIRE(bytes && n_tensors >= 0 && (sizes || !n_tensors), "sizes or bytes is NULL, or n_tensors negative");
-  *bytes = 8 * std::max<uint64_t>(1, chunks_of(n_tensors, sizes));
+  HB_HEAD_REQUIRE(bytes && n_tensors >= 0, "bytes is NULL or n_tensors negative");
+  *bytes = 8 * most_sums(n_tensors, sm_count(device));
   return HB_OK;
 }
 
@@ -164,11 +292,17 @@ hb_status hb_grad_norm(int32_t device, int32_t n_tensors, const void* const* ten
   begin_call();
   if (hb_status st = check_tensors(n_tensors, tensors, sizes, dtypes)) return st;
   HB_HEAD_REQUIRE(norm && aligned(norm, 4), "norm is NULL or not aligned");
-  HB_HEAD_REQUIRE(workspace && aligned(workspace, 8) && workspace_bytes >= 8 * std::max<uint64_t>(1, chunks_of(n_tensors, sizes)),
+  const int sms = sm_count(device);
+  HB_HEAD_REQUIRE(workspace && aligned(workspace, 8) && workspace_bytes >= 8 * most_sums(n_tensors, sms),
                   "workspace is too small or not 8-byte aligned");
   DeviceScope dev(device);
   if (!dev.ok()) return fail(HB_REFUSED, "no such device");
-  return norm_launch(n_tensors, tensors, sizes, dtypes, norm, (double*)workspace, (cudaStream_t)stream);
+  cudaStream_t s = (cudaStream_t)stream;
+  double* sums = (double*)workspace;
+  const uint32_t n = n_tensors <= kSmall ? sum_launches<kSmall>(n_tensors, tensors, sizes, dtypes, sums, sms, s)
+                                         : sum_launches<kLarge>(n_tensors, tensors, sizes, dtypes, sums, sms, s);
+  k_norm<<<1, kClipThreads, 0, s>>>(sums, n, norm);
+  return launched("hb_grad_norm");
 }
 
 hb_status hb_clip_grad_norm(int32_t device, int32_t n_tensors, const void* const* tensors, void* const* outs,
@@ -181,15 +315,25 @@ hb_status hb_clip_grad_norm(int32_t device, int32_t n_tensors, const void* const
   HB_HEAD_REQUIRE(outs || !n_tensors, "outs is NULL");
   for (int i = 0; i < n_tensors; ++i)
     HB_HEAD_REQUIRE((outs[i] || !sizes[i]) && aligned(outs[i], size_of(dtypes[i])), "an output is NULL or not aligned to its type");
-  HB_HEAD_REQUIRE(workspace && aligned(workspace, 8) && workspace_bytes >= 8 * std::max<uint64_t>(1, chunks_of(n_tensors, sizes)),
+  const int sms = sm_count(device);
+  HB_HEAD_REQUIRE(workspace && aligned(workspace, 8) && workspace_bytes >= 8 * most_sums(n_tensors, sms),
                   "workspace is too small or not 8-byte aligned");
   DeviceScope dev(device);
   if (!dev.ok()) return fail(HB_REFUSED, "no such device");
   cudaStream_t s = (cudaStream_t)stream;
-  if (hb_status st = norm_launch(n_tensors, tensors, sizes, dtypes, norm, (double*)workspace, s)) return st;
-  each_table(n_tensors, tensors, outs, sizes, dtypes, [&](const Table& t, uint32_t chunks, uint64_t) {
-    k_clip<<<chunks, kClipThreads, 0, s>>>(t, norm, max_norm);
-  });
+  double* sums = (double*)workspace;
+  const auto run = [&](auto table) {
+    constexpr int kTable = decltype(table)::value;
+    const uint32_t n = sum_launches<kTable>(n_tensors, tensors, sizes, dtypes, sums, sms, s);
+    float* to = norm;  // the first launch writes it
+    each_table<kTable>(n_tensors, tensors, outs, sizes, dtypes, sms, [&](const Table<kTable>& t, uint32_t ctas) {
+      k_clip<kTable><<<ctas, kClipThreads, 0, s>>>(t, sums, n, max_norm, to);
+      to = nullptr;
+    });
+    if (to) k_norm<<<1, kClipThreads, 0, s>>>(sums, n, norm);  // no element at all
+  };
+  if (n_tensors <= kSmall) run(std::integral_constant<int, kSmall>{});
+  else run(std::integral_constant<int, kLarge>{});
   return launched("hb_clip_grad_norm");
 }
 

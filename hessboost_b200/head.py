@@ -17,6 +17,7 @@ refuses raises HbError. Results do not change from run to run.
 """
 
 import ctypes
+import operator
 
 import torch
 
@@ -189,7 +190,8 @@ def layer_norm_forward(x, weight=None, bias=None, *, eps=1e-5):
     w = None if weight is None else weight.contiguous()
     b = None if bias is None else bias.contiguous()
     y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    mean, rstd = torch.empty((2, n), dtype=torch.float32, device=x.device).unbind(0)
+    mean = torch.empty(n, dtype=torch.float32, device=x.device)
+    rstd = torch.empty_like(mean)
     _check(lib().hb_layer_norm_forward(dev, rows.data_ptr(), dt, max(rows.stride(0), width), n, width,
                                        None if w is None else w.data_ptr(), None if b is None else b.data_ptr(), pt,
                                        eps, y.data_ptr(), mean.data_ptr(), rstd.data_ptr(), _stream(dev)),
@@ -279,27 +281,36 @@ def linear_xent_backward(dloss, x, weight, labels, lse):
 
 
 # -------------------------------------------------------------- clipping
+_of = operator.attrgetter
+_contiguous = operator.methodcaller("is_contiguous")
+_data_ptr = operator.methodcaller("data_ptr")
+_numel = operator.methodcaller("numel")
+
+
 def _tensor_list(tensors):
-    """The host arrays of a list of contiguous tensors on one device, and that device."""
+    """The host arrays of a list of contiguous tensors on one device, and that device. (Hundreds of tensors: each
+    question is asked of all of them in one call.)"""
     n = len(tensors)
     _need(n > 0, "tensors is empty")
-    dev = _device(*tensors)
-    for t in tensors:
-        _need(t.dtype in _TYPES, "tensors must be float32, float16 or bfloat16")
-        _need(t.is_contiguous(), "tensors must be contiguous")
-    ptrs = (ctypes.c_void_p * n)(*[t.data_ptr() for t in tensors])
-    sizes = (ctypes.c_uint64 * n)(*[t.numel() for t in tensors])
-    types = (ctypes.c_int32 * n)(*[_TYPES[t.dtype] for t in tensors])
-    return n, ptrs, sizes, types, dev
+    devices = set(map(_of("device"), tensors))
+    _need(len(devices) == 1, "tensors must be on one device")
+    device = devices.pop()
+    _need(device.type == "cuda", "tensors must be on a CUDA device")
+    _need(all(map(_contiguous, tensors)), "tensors must be contiguous")
+    dtypes = list(map(_of("dtype"), tensors))
+    _need(_TYPES.keys() >= set(dtypes), "tensors must be float32, float16 or bfloat16")
+    sizes = list(map(_numel, tensors))
+    return (n, (ctypes.c_void_p * n)(*map(_data_ptr, tensors)), (ctypes.c_uint64 * n)(*sizes),
+            (ctypes.c_int32 * n)(*map(_TYPES.__getitem__, dtypes)), device.index, sizes, dtypes)
 
 
 def grad_norm(tensors):
     """The 2-norm of all the tensors' elements together, a float32 scalar tensor on their device."""
     tensors = list(tensors)
-    n, ptrs, sizes, types, dev = _tensor_list(tensors)
+    n, ptrs, sizes, types, dev, _, _ = _tensor_list(tensors)
     L = lib()
     norm = torch.empty((), dtype=torch.float32, device=tensors[0].device)
-    ws, size = _workspace(L.hb_grad_norm_workspace, norm.device, n, sizes)
+    ws, size = _workspace(L.hb_grad_norm_workspace, norm.device, dev, n)
     _check(L.hb_grad_norm(dev, n, ptrs, sizes, types, norm.data_ptr(), ws.data_ptr(), size, _stream(dev)),
            "hb_grad_norm")
     return norm
@@ -311,19 +322,18 @@ def clip_grad_norm(tensors, max_norm, *, out=None):
     the results through that factor."""
     tensors = list(tensors)
     _need(max_norm >= 0, "max_norm must be >= 0")
-    n, ptrs, sizes, types, dev = _tensor_list(tensors)
+    n, ptrs, sizes, types, dev, numels, dtypes = _tensor_list(tensors)
     outs = ptrs
     if out is not None:
         out = list(out)
         _need(len(out) == n, "out must have a tensor for each of tensors")
-        _device(tensors[0], *out)
-        for t, o in zip(tensors, out):
-            _need(o.dtype == t.dtype and o.numel() == t.numel() and o.is_contiguous(),
-                  "out must be contiguous tensors of the same sizes and types")
-        outs = (ctypes.c_void_p * n)(*[o.data_ptr() for o in out])
+        _need(set(map(_of("device"), out)) == {tensors[0].device}, "tensors must be on one device")
+        _need(list(map(_numel, out)) == numels and list(map(_of("dtype"), out)) == dtypes and all(map(_contiguous, out)),
+              "out must be contiguous tensors of the same sizes and types")
+        outs = (ctypes.c_void_p * n)(*map(_data_ptr, out))
     L = lib()
     norm = torch.empty((), dtype=torch.float32, device=tensors[0].device)
-    ws, size = _workspace(L.hb_grad_norm_workspace, norm.device, n, sizes)
+    ws, size = _workspace(L.hb_grad_norm_workspace, norm.device, dev, n)
     _check(L.hb_clip_grad_norm(dev, n, ptrs, outs, sizes, types, max_norm, norm.data_ptr(), ws.data_ptr(), size,
                                _stream(dev)), "hb_clip_grad_norm")
     return norm

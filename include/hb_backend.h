@@ -521,7 +521,7 @@ hb_status hb_linear_xent_backward(int32_t device, const float* dloss, uint64_t d
 /* *norm (device, f32) = the 2-norm of all the tensors' elements together.
  * `tensors`, `sizes` (elements) and `dtypes` are host arrays, read before
  * the call returns; tensors[i] is contiguous device memory. */
-hb_status hb_grad_norm_workspace(int32_t n_tensors, const uint64_t* sizes, uint64_t* bytes);
+hb_status hb_grad_norm_workspace(int32_t device, int32_t n_tensors, uint64_t* bytes);
 hb_status hb_grad_norm(int32_t device, int32_t n_tensors, const void* const* tensors, const uint64_t* sizes,
                        const int32_t* dtypes, float* norm, void* workspace, uint64_t workspace_bytes,
                        void* stream);

@@ -191,7 +191,7 @@ extern "C" {
         label_type: i32, lse: *const f32, n_rows: u64, width: u32, n_classes: u64, dx: *mut c_void,
         dw: *mut c_void, workspace: *mut c_void, workspace_bytes: u64, stream: *mut c_void) ->
         hb_status;
-    pub fn hb_grad_norm_workspace(n_tensors: i32, sizes: *const u64, bytes: *mut u64) -> hb_status;
+    pub fn hb_grad_norm_workspace(device: i32, n_tensors: i32, bytes: *mut u64) -> hb_status;
     pub fn hb_grad_norm(device: i32, n_tensors: i32, tensors: *const *const c_void, sizes: *const
         u64, dtypes: *const i32, norm: *mut f32, workspace: *mut c_void, workspace_bytes: u64,
         stream: *mut c_void) -> hb_status;

@@ -79,7 +79,7 @@ def test_clip_refusals():
                         (3, (ctypes.c_void_p * 1)(P + 2), "aligned"), (5, (ctypes.c_int32 * 1)(7), "type"),
                         (4, (ctypes.c_uint64 * 1)(2**50), "large")):
         refused("hb_clip_grad_norm", put(ok, at, v), what)
-    refused("hb_grad_norm_workspace", [1, None, ctypes.c_uint64()], "NULL")
+    refused("hb_grad_norm_workspace", [0, 1, None], "NULL")
     refused("hb_grad_norm", [0, 1, one, size, types, Q + 1, P, 1 << 20, None], "norm")
 
 
