@@ -8,11 +8,11 @@
 // rest of the sum f64, in an order that the sizes alone decide.
 //
 // Bound by memory: everything is read, and for clipping read again and
-// written. Tensors are cut into chunks of 1,024 vectors of 16 bytes, and each
-// CTA takes a run of chunks, whatever the tensors' sizes. The second reading
-// goes through each run backwards: what the first one left in the L2 cache is
-// its end. Clipping has no kernel for the norm between the two: every CTA adds
-// the first kernel's sums itself.
+// written. Tensors are cut into chunks of 1,024 vectors of 16 bytes, dealt to
+// the CTAs in turn, whatever the tensors' sizes (a CTA with a run of chunks of
+// its own kept to 3.4 TB/s). The second reading goes backwards: what the first
+// one left in the L2 cache is the end. Clipping has no kernel for the norm
+// between the two: every CTA adds the first kernel's sums itself.
 #include <algorithm>
 
 #include "hb_head.h"
@@ -25,7 +25,7 @@ constexpr int kClipThreads = 256;
 constexpr int kEach = 4;                               // vectors a thread of a chunk
 constexpr uint32_t kChunk = kClipThreads * kEach;      // vectors
 constexpr int kSmall = 24, kLarge = 512;               // tensors of a launch
-constexpr int kCtasPerSm = 8;
+constexpr int kCtasPerSm = 4;                          // all there at once, by their registers
 
 // The tensors of a launch, passed as a kernel argument (no device copy of
 // the table). first[i] = chunks before tensor i.
@@ -38,16 +38,6 @@ struct Table {
   uint8_t dtype[kTable];
   int count;
 };
-
-template <int kTable>
-__device__ __forceinline__ int tensor_of(const Table<kTable>& t, uint32_t chunk) {
-  int lo = 0, hi = t.count - 1;  // last tensor whose first chunk is <= chunk
-  while (lo < hi) {
-    const int m = (lo + hi + 1) >> 1;
-    if (t.first[m] <= chunk) lo = m; else hi = m - 1;
-  }
-  return lo;
-}
 
 // A tensor's vectors: elements [head, head + V count) on 16-byte boundaries
 // of `at`, of which in[] is `shift` elements past such a boundary. With a
@@ -106,23 +96,25 @@ template <typename T>
 __device__ __forceinline__ float squares(const T* in, uint64_t n, uint32_t chunk) {
   constexpr int V = 16 / sizeof(T);
   const Span s = span_of(in, in, n);
+  const Pack<T, V>* from = reinterpret_cast<const Pack<T, V>*>(in + s.head) + (uint64_t)chunk * kChunk + threadIdx.x;
+  const int64_t left = (int64_t)s.count - (int64_t)((uint64_t)chunk * kChunk + threadIdx.x);
   float acc[4] = {};
-  Pack<T, V> q[kEach];
+  const auto add = [&](const Pack<T, V>& q) {
 #pragma unroll
-  for (int i = 0; i < kEach; ++i) {
-    const uint64_t j = (uint64_t)chunk * kChunk + i * kClipThreads + threadIdx.x;
-    if (j < s.count) q[i] = reinterpret_cast<const Pack<T, V>*>(in + s.head)[j];
-  }
-#pragma unroll
-  for (int i = 0; i < kEach; ++i) {
-    const uint64_t j = (uint64_t)chunk * kChunk + i * kClipThreads + threadIdx.x;
-    if (j < s.count) {
-#pragma unroll
-      for (int k = 0; k < V; ++k) {
-        const float x = to_f32(q[i].v[k]);
-        acc[k & 3] = fmaf(x, x, acc[k & 3]);
-      }
+    for (int k = 0; k < V; ++k) {
+      const float x = to_f32(q.v[k]);
+      acc[k & 3] = fmaf(x, x, acc[k & 3]);
     }
+  };
+  if ((uint64_t)(chunk + 1) * kChunk <= s.count) {  // a whole chunk: its loads go out together
+    Pack<T, V> q[kEach];
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) q[i] = from[i * kClipThreads];
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) add(q[i]);
+  } else {
+    for (int i = 0; i < kEach; ++i)
+      if (i * kClipThreads < left) add(from[i * kClipThreads]);
   }
   if (chunk == 0) {
     const uint64_t ends = n - s.count * V;  // single elements: s.head before the vectors, the others after
@@ -135,12 +127,11 @@ __device__ __forceinline__ float squares(const T* in, uint64_t n, uint32_t chunk
 }
 
 template <int kTable>
-__global__ void __launch_bounds__(kClipThreads) k_square_sums(const __grid_constant__ Table<kTable> t, double* __restrict__ sums) {
+__global__ void __launch_bounds__(kClipThreads, kCtasPerSm) k_square_sums(const __grid_constant__ Table<kTable> t, double* __restrict__ sums) {
   const uint32_t chunks = t.first[t.count];
-  const uint32_t c0 = (uint32_t)((uint64_t)chunks * blockIdx.x / gridDim.x), c1 = (uint32_t)((uint64_t)chunks * (blockIdx.x + 1) / gridDim.x);
   double v = 0.0;
-  int i = tensor_of(t, c0);
-  for (uint32_t c = c0; c < c1; ++c) {
+  int i = 0;
+  for (uint32_t c = blockIdx.x; c < chunks; c += gridDim.x) {
     while (c >= t.first[i + 1]) ++i;
     const uint32_t k = c - t.first[i];
     v += (double)(t.dtype[i] == HB_F32   ? squares((const float*)t.in[i], t.n[i], k)
@@ -167,26 +158,34 @@ template <typename T>
 __device__ __forceinline__ void scale_chunk(const T* in, T* out, uint64_t n, uint32_t chunk, float by) {
   constexpr int V = 16 / sizeof(T);
   const Span s = span_of(in, out, n);
-  const uint4* units = reinterpret_cast<const uint4*>(in + s.head - s.shift);
-  uint4 a[kEach], b[kEach];
+  const uint64_t first = (uint64_t)chunk * kChunk + threadIdx.x;
+  const uint4* from = reinterpret_cast<const uint4*>(in + s.head - s.shift) + first;
+  uint4* to = reinterpret_cast<uint4*>(out + s.head) + first;
+  const uint32_t shift = s.shift * sizeof(T);
+  const auto put = [&](int i, uint4 u) {
+    Pack<T, V>& q = reinterpret_cast<Pack<T, V>&>(u);
 #pragma unroll
-  for (int i = 0; i < kEach; ++i) {
-    const uint64_t j = (uint64_t)chunk * kChunk + i * kClipThreads + threadIdx.x;
-    if (j < s.count) {
-      a[i] = units[j];
-      if (s.shift) b[i] = units[j + 1];
+    for (int k = 0; k < V; ++k) q.v[k] = from_f32<T>(to_f32(q.v[k]) * by);
+    __stcs(to + i * kClipThreads, u);  // not read again: the cache is for what is
+  };
+  if ((uint64_t)(chunk + 1) * kChunk <= s.count) {
+    uint4 a[kEach], b[kEach];
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) a[i] = from[i * kClipThreads];
+    if (shift) {
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) b[i] = from[i * kClipThreads + 1];
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) a[i] = shifted(a[i], b[i], shift);
     }
-  }
 #pragma unroll
-  for (int i = 0; i < kEach; ++i) {
-    const uint64_t j = (uint64_t)chunk * kChunk + i * kClipThreads + threadIdx.x;
-    if (j < s.count) {
-      uint4 u = s.shift ? shifted(a[i], b[i], s.shift * sizeof(T)) : a[i];
-      Pack<T, V>& q = reinterpret_cast<Pack<T, V>&>(u);
-#pragma unroll
-      for (int k = 0; k < V; ++k) q.v[k] = from_f32<T>(to_f32(q.v[k]) * by);
-      __stcs(reinterpret_cast<uint4*>(out + s.head) + j, u);  // not read again: the cache is for what is
-    }
+    for (int i = 0; i < kEach; ++i) put(i, a[i]);
+  } else {
+    for (int i = 0; i < kEach; ++i)
+      if (first + i * kClipThreads < s.count) {
+        const uint4 a = from[i * kClipThreads];
+        put(i, shift ? shifted(a, from[i * kClipThreads + 1], shift) : a);
+      }
   }
   if (chunk == 0) {
     const uint64_t ends = n - s.count * V;
@@ -200,17 +199,16 @@ __device__ __forceinline__ void scale_chunk(const T* in, T* out, uint64_t n, uin
 // out = in for a launch's tensors, scaled by the norm of all launches' sums;
 // in and out may be the same tensors.
 template <int kTable>
-__global__ void __launch_bounds__(kClipThreads)
+__global__ void __launch_bounds__(kClipThreads, kCtasPerSm)
     k_clip(const __grid_constant__ Table<kTable> t, const double* __restrict__ sums, uint32_t n_sums, float max_norm, float* __restrict__ norm) {
   const float all = norm_of(sums, n_sums);
   if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = all;
   const float q = max_norm / (all + 1e-6f);
   const float by = q > 1.0f ? 1.0f : q;  // NaN stays NaN
   const uint32_t chunks = t.first[t.count];
-  const uint32_t c0 = (uint32_t)((uint64_t)chunks * blockIdx.x / gridDim.x), c1 = (uint32_t)((uint64_t)chunks * (blockIdx.x + 1) / gridDim.x);
-  if (c0 == c1) return;
-  int i = tensor_of(t, c1 - 1);
-  for (uint32_t c = c1; c-- > c0;) {
+  int i = t.count - 1;
+  for (uint32_t back = blockIdx.x; back < chunks; back += gridDim.x) {
+    const uint32_t c = chunks - 1 - back;
     while (c < t.first[i]) --i;
     const uint32_t k = c - t.first[i];
     if (t.dtype[i] == HB_F32) scale_chunk((const float*)t.in[i], (float*)t.out[i], t.n[i], k, by);
