@@ -14,7 +14,8 @@ CSRC = os.path.join(HERE, "csrc")
 OUT_DIR = os.path.join(HERE, "_lib")
 LIB = os.path.join(OUT_DIR, "libhb_cuda.so")
 SOURCES = ["hb_kernels.cu", "hb_engine.cu", "hb_peer.cu", "hb_predict.cu", "hb_noalloc.cu", "hb_probe.cu", "hb_sketch.cu",
-           "hb_head.cu", "hb_embed.cu", "hb_norm.cu", "hb_xent.cu", "hb_xent_mma.cu", "hb_clip.cu",
+           "hb_head.cu", "hb_embed.cu", "hb_norm.cu", "hb_xent.cu", "hb_xent_mma.cu", "hb_xent_few.cu",
+           "hb_clip.cu",
            "hb_host_bins.cpp", "hb_model_io.cpp"]
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 FLAGS = [

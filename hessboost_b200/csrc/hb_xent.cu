@@ -166,15 +166,25 @@ int tile_cols(uint64_t cols, uint64_t m_tiles, int workers, int unit) {
   uint64_t n = (cols + 255) / 256;
   while (m_tiles * n < (uint64_t)workers && (cols + n) / (n + 1) > 64) ++n;
   const auto size = [&](uint64_t k) { return round_up((cols + k - 1) / k, unit); };
-  // one tile more where that leaves much less of the last one empty
-  if (5 * (n + 1) * size(n + 1) <= 4 * n * size(n)) ++n;
   return (int)size(n);
 }
-// Parts of k: enough tiles for the workers, at least 4 steps of 64 each.
-int k_splits(uint64_t tiles, int k_blocks, int workers) {
-  if (tiles >= (uint64_t)workers) return 1;
-  const int want = (int)((workers + tiles - 1) / tiles);
-  return std::max(1, std::min(want, k_blocks * kMmaDepth / 4));
+// Columns of the last of the tiles of n columns: 16 a CTA, 32, 64, or all,
+// where that is enough (each CTA's share then lies in whole blocks of 64, or
+// inside one).
+int last_cols(uint64_t cols, int n, bool pair) {
+  const int ctas = pair ? 2 : 1, left = (int)((cols - 1) % n + 1);
+  for (int share : {16, 32, 64})
+    if (share * ctas >= left && share * ctas <= n) return share * ctas;
+  return n;
+}
+// Parts of k: enough tiles for the workers, at least 4 steps of 64 each. In
+// f32 a part is at most 2,048 long: the tensor cores' own sums round towards
+// zero, and over 4,099 rows that was 2e-6 of dw, twice what f32 sums that
+// round to nearest are off.
+int k_splits(uint64_t tiles, int k_blocks, int workers, int planes) {
+  const int want = tiles >= (uint64_t)workers ? 1 : (int)((workers + tiles - 1) / tiles);
+  const int by_tiles = std::max(1, std::min(want, k_blocks * kMmaDepth / 4));
+  return planes == 1 ? by_tiles : std::max(by_tiles, std::min(32, (k_blocks * kMmaDepth * 64 + 2047) / 2048));
 }
 
 struct Forward {
@@ -215,9 +225,10 @@ Backward backward_plan(const Sizes& z, int32_t dtype, const void* x, uint64_t x_
   b.x = operand_of(z, dtype, x, x_stride, z.n_rows, true);
   b.w = operand_of(z, dtype, w, w_stride, z.n_classes, false);
   const uint64_t most = (uint64_t)kGradElements / z.planes;
-  const uint64_t least = 4096;  // classes of a piece, where there are as many
+  const uint64_t least = 2048;  // classes of a piece, where there are as many
   b.chunk = std::min(z.n_rows, std::max<uint64_t>(most / std::min(z.n_classes, least) / 256 * 256, 256));
   b.chunks = (z.n_rows + b.chunk - 1) / b.chunk;
+  b.chunk = std::min(b.chunk, round_up((z.n_rows + b.chunks - 1) / b.chunks, 256));
   b.piece = std::min(z.n_classes, std::max<uint64_t>(most / b.chunk / 256 * 256, 256));
   b.pieces = (z.n_classes + b.piece - 1) / b.piece;
   b.piece = std::min(b.piece, round_up((z.n_classes + b.pieces - 1) / b.pieces, 256));
@@ -227,9 +238,11 @@ Backward backward_plan(const Sizes& z, int32_t dtype, const void* x, uint64_t x_
   const uint64_t row_tiles = (b.chunk + m - 1) / m, class_tiles = (b.piece + m - 1) / m;
   b.grad_n = tile_cols(b.piece, row_tiles, workers, b.pair ? 128 : 64);
   b.out_n = tile_cols(z.width, row_tiles + class_tiles, workers, b.pair ? 128 : 64);
+  // two tiles of which one would be mostly empty: whole ones and a narrow last
+  if (z.width > 256 && z.width % 256 <= 128) b.out_n = 256;
   const uint64_t out_tiles = (z.width + b.out_n - 1) / b.out_n;
-  b.dx_splits = k_splits(row_tiles * out_tiles, stages_of(b.piece), workers);
-  b.dw_splits = k_splits(class_tiles * out_tiles, stages_of(b.chunk), workers);
+  b.dx_splits = k_splits(row_tiles * out_tiles, stages_of(b.piece), workers, z.planes);
+  b.dw_splits = k_splits(class_tiles * out_tiles, stages_of(b.chunk), workers, z.planes);
   b.dx_acc = b.dx_splits > 1 || b.pieces > 1;
   b.dw_acc = b.dw_splits > 1 || b.chunks > 1;
   b.acc_stride = (uint32_t)round_up(z.width, 4);
@@ -310,7 +323,7 @@ hb_status hb_linear_xent_forward_workspace(int32_t device, const void* x, uint64
   begin_call();
   if (hb_status st = check_xent(x, x_stride, w, w_stride, dtype, n_rows, width, n_classes)) return st;
   HB_HEAD_REQUIRE(bytes, "bytes is NULL");
-  *bytes = n_rows ? forward_plan(sizes_of(dtype, n_rows, width, n_classes), dtype, x, x_stride, w, w_stride, sm_count(device)).bytes : 0;
+  *bytes = !n_rows || few_applies(dtype, width, n_classes) ? 0 : forward_plan(sizes_of(dtype, n_rows, width, n_classes), dtype, x, x_stride, w, w_stride, sm_count(device)).bytes;
   return HB_OK;
 }
 
@@ -325,6 +338,13 @@ hb_status hb_linear_xent_forward(int32_t device, const void* x, uint64_t x_strid
   HB_HEAD_REQUIRE(loss && lse && aligned(loss, 4) && aligned(lse, 4), "loss or lse is NULL or not aligned");
   const Sizes z = sizes_of(dtype, n_rows, width, n_classes);
   const int sms = sm_count(device);
+  if (few_applies(dtype, width, n_classes)) {
+    DeviceScope dev(device);
+    if (!dev.ok()) return fail(HB_REFUSED, "no such device");
+    few_forward(XentCall{x, w, labels, x_stride, w_stride, n_rows, n_classes, width, label_type}, loss, lse, device, sms,
+                (cudaStream_t)stream);
+    return launched("hb_linear_xent_forward");
+  }
   const Forward f = forward_plan(z, dtype, x, x_stride, w, w_stride, sms);
   HB_HEAD_REQUIRE(workspace && aligned(workspace, 256) && workspace_bytes >= f.bytes,
                   "workspace is too small or not 256-byte aligned");
@@ -350,7 +370,7 @@ hb_status hb_linear_xent_forward(int32_t device, const void* x, uint64_t x_strid
   for (uint64_t r0 = 0; r0 < n_rows; r0 += f.chunk) {
     const uint64_t rows = std::min(f.chunk, n_rows - r0);
     p.part_stride = rows;
-    p.jobs[0] = MmaJob{kJobStats, (int)((rows + m - 1) / m), f.n_tiles, f.n_size, (int)width, stages_of(width), 1, 1,
+    p.jobs[0] = MmaJob{kJobStats, (int)((rows + m - 1) / m), f.n_tiles, f.n_size, f.n_size, (int)width, stages_of(width), 1, 1,
                        (int)r0, (int)rows, 0, (int)n_classes, {}};
     if (hb_status st = mma_launch(p, f.pair, sms, s)) return st;
     with_xent_types(dtype, label_type, [&](auto, auto l) {
@@ -368,7 +388,11 @@ hb_status hb_linear_xent_backward_workspace(int32_t device, const void* x, uint6
   begin_call();
   if (hb_status st = check_xent(x, x_stride, w, w_stride, dtype, n_rows, width, n_classes)) return st;
   HB_HEAD_REQUIRE(bytes, "bytes is NULL");
-  *bytes = n_rows ? backward_plan(sizes_of(dtype, n_rows, width, n_classes), dtype, x, x_stride, w, w_stride, sm_count(device)).bytes : 0;
+  const int sms = sm_count(device);
+  *bytes = !n_rows ? 0
+           : few_applies(dtype, width, n_classes)
+               ? few_bytes(n_rows, width, n_classes, sms)
+               : backward_plan(sizes_of(dtype, n_rows, width, n_classes), dtype, x, x_stride, w, w_stride, sms).bytes;
   return HB_OK;
 }
 
@@ -385,6 +409,16 @@ hb_status hb_linear_xent_backward(int32_t device, const float* dloss, uint64_t d
                   "a buffer is not aligned to its type");
   const Sizes z = sizes_of(dtype, n_rows, width, n_classes);
   const int sms = sm_count(device);
+  if (n_rows && few_applies(dtype, width, n_classes)) {
+    const uint64_t bytes = few_bytes(n_rows, width, n_classes, sms);
+    HB_HEAD_REQUIRE(!bytes || (workspace && aligned(workspace, 256) && workspace_bytes >= bytes),
+                    "workspace is too small or not 256-byte aligned");
+    DeviceScope dev(device);
+    if (!dev.ok()) return fail(HB_REFUSED, "no such device");
+    few_backward(XentCall{x, w, labels, x_stride, w_stride, n_rows, n_classes, width, label_type}, dloss, dloss_stride, lse, dx, dw,
+                 workspace, device, sms, (cudaStream_t)stream);
+    return launched("hb_linear_xent_backward");
+  }
   Backward b{};
   if (n_rows) {
     b = backward_plan(z, dtype, x, x_stride, w, w_stride, sms);
@@ -422,7 +456,7 @@ hb_status hb_linear_xent_backward(int32_t device, const float* dloss, uint64_t d
   p.lse = lse;
   const uint64_t e = size_of(dtype);
   const int out_type = dtype == HB_F32 ? kOutF32 : kOutBf16, m = b.pair ? 256 : 128;
-  const int out_tiles = (int)((width + b.out_n - 1) / b.out_n);
+  const int out_tiles = (int)((width + b.out_n - 1) / b.out_n), last = last_cols(width, b.out_n, b.pair);
   const auto vec = [&](const void* q) { return (int)(aligned(q, 16) && width * e % 16 == 0 && b.out_n * e % 16 == 0); };
   // dx or dw of `rows` rows from `splits` accumulators
   const auto finish = [&](const float* acc, int splits, uint64_t split_rows, uint64_t rows, void* to) {
@@ -459,10 +493,12 @@ hb_status hb_linear_xent_backward(int32_t device, const float* dloss, uint64_t d
       // a last piece or chunk may have fewer steps of k than splits: the
       // splits without any add 0
       MmaJob& jw = p.jobs[p.n_jobs++] = done;
+      jw.n_last = last;
       jw.kind = kJobDw, jw.m_tiles = (done.n_classes + m - 1) / m, jw.n_tiles = out_tiles, jw.n_size = b.out_n;
       jw.k_total = done.n_rows, jw.k_blocks = stages_of(done.n_rows), jw.splits = b.dw_splits;
       jw.out = MmaOut{b.dw_acc ? kOutAcc : out_type, c > 0, vec(dw_to), (int)b.dw_rows, (int)b.acc_stride, acc, dw_to};
       MmaJob& jx = p.jobs[p.n_jobs++] = done;
+      jx.n_last = last;
       jx.kind = kJobDx, jx.m_tiles = (done.n_rows + m - 1) / m, jx.n_tiles = out_tiles, jx.n_size = b.out_n;
       jx.k_total = done.n_classes, jx.k_blocks = stages_of(done.n_classes), jx.splits = b.dx_splits;
       jx.out = MmaOut{b.dx_acc ? kOutAcc : out_type, q > 0, vec(dx_to), (int)b.chunk, (int)b.acc_stride, dx_acc, dx_to};
@@ -472,7 +508,7 @@ hb_status hb_linear_xent_backward(int32_t device, const float* dloss, uint64_t d
       sizes(jg, i);
       if (!g_lay(jg, i).map(&p.g_out, 32, 1)) return fail(HB_DEVICE_FAILED, "tensor map");
       jg.kind = kJobGrad, jg.m_tiles = (jg.n_rows + m - 1) / m, jg.n_tiles = (jg.n_classes + b.grad_n - 1) / b.grad_n;
-      jg.n_size = b.grad_n, jg.k_total = (int)width, jg.k_blocks = stages_of(width), jg.splits = 1, jg.m_fast = 1;
+      jg.n_size = jg.n_last = b.grad_n, jg.k_total = (int)width, jg.k_blocks = stages_of(width), jg.splits = 1, jg.m_fast = 1;
     }
     if (hb_status st = mma_launch(p, b.pair, sms, s)) return st;
     if (i > 0 && b.dw_acc && c + 1 == b.chunks) finish(acc, b.dw_splits, b.dw_rows, done.n_classes, dw_to);

@@ -24,12 +24,12 @@ struct MmaOut {
 
 constexpr int kMmaDepth = 2;  // blocks of 64 of k in a stage
 
-// m_tiles x n_tiles tiles of (128 x CTAs) x n_size, k (k_total of it) in
+// m_tiles x n_tiles tiles of (128 x CTAs) x n_size (the last ones n_last), k (k_total of it) in
 // k_blocks stages shared among `splits` tiles each; m_fast: consecutive tiles go down the rows.
 // The job's rows are [row0, row0 + n_rows) of the call's, its classes
 // [class0, class0 + n_classes) of the layer's.
 struct MmaJob {
-  int kind, m_tiles, n_tiles, n_size, k_total, k_blocks, splits, m_fast;
+  int kind, m_tiles, n_tiles, n_size, n_last, k_total, k_blocks, splits, m_fast;
   int row0, n_rows, class0, n_classes;
   MmaOut out;
 };
@@ -72,6 +72,24 @@ bool mma_map(CUtensorMap* map, const void* p, uint64_t blocks, uint64_t rows, ui
              uint64_t plane_stride, int box_rows, int box_blocks);
 // Runs the jobs by single CTAs or (pair) by pairs of them; shares the tiles out.
 hb_status mma_launch(MmaParams& p, bool pair, int sms, cudaStream_t s);
+
+// ---- few classes (hb_xent_few.cu) -------------------------------------------
+
+// x, w and the labels of a call.
+struct XentCall {
+  const void *x, *w, *labels;
+  uint64_t x_stride, w_stride, n_rows, n_classes;
+  uint32_t width;
+  int32_t label_type;
+};
+
+// Whether the layer is one for these (a rule on its sizes).
+bool few_applies(int32_t dtype, uint32_t width, uint64_t n_classes);
+// Workspace of the backward call.
+uint64_t few_bytes(uint64_t n_rows, uint32_t width, uint64_t n_classes, int sms);
+void few_forward(const XentCall& c, float* loss, float* lse, int device, int sms, cudaStream_t s);
+void few_backward(const XentCall& c, const float* dloss, uint64_t dloss_stride, const float* lse, void* dx, void* dw, void* workspace,
+                  int device, int sms, cudaStream_t s);
 
 }  // namespace head
 }  // namespace hb

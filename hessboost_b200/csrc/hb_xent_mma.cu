@@ -78,7 +78,7 @@ struct Ring {
 };
 
 struct TileAt {
-  int m, n, k0, k1, split;  // k in stages
+  int m, n, cols, k0, k1, split;  // k in stages
 };
 
 __device__ __forceinline__ TileAt tile_at(const MmaJob& job, int t) {
@@ -88,6 +88,7 @@ __device__ __forceinline__ TileAt tile_at(const MmaJob& job, int t) {
   t -= a.split * plane;
   if (job.m_fast) a.n = t / job.m_tiles, a.m = t - a.n * job.m_tiles;
   else a.m = t / job.n_tiles, a.n = t - a.m * job.n_tiles;
+  a.cols = a.n + 1 == job.n_tiles ? job.n_last : job.n_size;
   a.k0 = (int)((long long)job.k_blocks * a.split / job.splits);
   a.k1 = (int)((long long)job.k_blocks * (a.split + 1) / job.splits);
   return a;
@@ -157,11 +158,12 @@ __global__ void __launch_bounds__(kThreads, 1) k_xent_mma(const __grid_constant_
     uint32_t issued = 0;  // stages with a copy in flight or landed
     bool ok = true;
     each_tile(p, worker, [&](const MmaJob& job, const TileAt& at) {
-      const int share = job.n_size / S::kCtas;  // this CTA's rows of B
+      const int share = at.cols / S::kCtas;  // this CTA's rows of B
       const bool a_mn = job.kind == kJobDw, b_mn = job.kind == kJobDx || job.kind == kJobDw;
       const CUtensorMap* ma = job.kind == kJobDw ? &p.g_mn : job.kind == kJobDx ? &p.g_k : &p.x_k;
       const CUtensorMap* mb = job.kind == kJobDw ? &p.x_mn : job.kind == kJobDx ? &p.w_mn : &p.w_k;
-      const uint32_t bytes = S::kABytes + share * kRow * kMmaDepth;
+      // a copy is of the whole tile's share, whatever lies past the last one's
+      const uint32_t bytes = S::kABytes + job.n_size / S::kCtas * kRow * kMmaDepth;
       // rows of the operands in their tensors: x starts at the job's first
       // row and w at its first class where those are its rows or its k
       const int a_row = (at.m * S::kCtas + rank) * 128 + (ma == &p.x_k ? job.row0 : 0);
@@ -178,7 +180,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_xent_mma(const __grid_constant_
           // coordinates: column in the block, row, block, plane
           if (a_mn) tma_load<kPair>(dst, ma, bar, 0, k * 64 * kMmaDepth, a_row >> 6, pa);
           else tma_load<kPair>(dst, ma, bar, 0, a_row, k * kMmaDepth, pa);
-          if (b_mn) tma_load<kPair>(dst + S::kABytes, mb, bar, 0, bk0 + k * 64 * kMmaDepth, b_row >> 6, pb);
+          if (b_mn) tma_load<kPair>(dst + S::kABytes, mb, bar, b_row & 63, bk0 + k * 64 * kMmaDepth, b_row >> 6, pb);
           else tma_load<kPair>(dst + S::kABytes, mb, bar, 0, b_row, k * kMmaDepth, pb);
           r.next();
         }
@@ -200,7 +202,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_xent_mma(const __grid_constant_
     int tile = 0;
     each_tile(p, worker, [&](const MmaJob& job, const TileAt& at) {
       const bool a_mn = job.kind == kJobDw, b_mn = job.kind == kJobDx || job.kind == kJobDw;
-      const uint32_t idesc = instr_desc(128 * S::kCtas, job.n_size, a_mn, b_mn), sa = k_step(a_mn), sb = k_step(b_mn);
+      const uint32_t idesc = instr_desc(128 * S::kCtas, at.cols, a_mn, b_mn), sa = k_step(a_mn), sb = k_step(b_mn);
       const int buf = tile & 1;
       if (!bar_wait<kPair>(acc_empty(buf), ((tile >> 1) & 1) ^ 1, &s_gave_up)) return false;
       fence_after();
@@ -208,7 +210,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_xent_mma(const __grid_constant_
       bool add = false;
       // k-major: 16 of k are 32 bytes on, the next block of 64 one block of
       // rows on; mn-major: 16 of k are 16 rows of 128 bytes on
-      const uint32_t share = job.n_size / S::kCtas;
+      const uint32_t share = job.n_size / S::kCtas;  // k-major tiles are all alike
       const uint32_t block_a = a_mn ? 64 * kRow >> 4 : 128 * kRow >> 4, block_b = b_mn ? 64 * kRow >> 4 : share * kRow >> 4;
       for (int q = 0; q < kPairs; ++q)
         for (int k = at.k0; k < at.k1; ++k) {
@@ -245,7 +247,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_xent_mma(const __grid_constant_
       const uint32_t acc = tmem + buf * 256 + ((uint32_t)(quarter * 32) << 16);
       const int row0 = (at.m * S::kCtas + rank) * 128 + quarter * 32, row = row0 + lane;
       const int col0 = at.n * job.n_size;
-      const int cut = (job.n_size / 2 + 63) & ~63, c0 = half ? cut : 0, c1 = half ? job.n_size : cut;
+      const int cut = min(at.cols, (at.cols / 2 + 63) & ~63), c0 = half ? cut : 0, c1 = half ? at.cols : cut;
       if (job.kind == kJobStats) {
         const bool in = row < job.n_rows;
         const int64_t rel = (in ? p.label((int64_t)job.row0 + row) : -1) - job.class0 - col0;

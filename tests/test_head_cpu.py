@@ -55,13 +55,13 @@ def test_norm_refusals():
 
 
 def test_xent_refusals():
-    ok = [0, P, 8, P, 8, 0, P, 0, 4, 8, 10, Q, Q, P, 1 << 30, None]
+    ok = [0, P, 8, P, 8, 0, P, 0, 4, 8, 100, Q, Q, P, 1 << 30, None]
     for at, v, what in ((5, 1, "f32 or bf16"), (7, 2, "label type"), (9, 0, "width"), (9, 2**21, "width"), (10, 0, "n_classes"),
                         (10, 2**31, "n_classes"), (8, 2**31, "rows"), (1, None, "NULL"), (3, None, "NULL"), (6, None, "NULL"),
                         (2, 7, "x_stride"), (4, 7, "w_stride"), (1, P + 2, "aligned"), (11, None, "NULL"), (12, Q + 2, "aligned"),
                         (13, None, "workspace"), (14, 1, "workspace")):
         refused("hb_linear_xent_forward", put(ok, at, v), what)
-    ok = [0, P, 1, P, 8, P, 8, 0, P, 0, P, 4, 8, 10, Q, Q, P, 1 << 30, None]
+    ok = [0, P, 1, P, 8, P, 8, 0, P, 0, P, 4, 8, 100, Q, Q, P, 1 << 30, None]
     for at, v, what in ((7, 1, "f32 or bf16"), (1, None, "NULL"), (10, None, "NULL"), (14, None, "NULL"), (15, None, "NULL"),
                         (1, P + 2, "aligned"), (16, None, "workspace"), (17, 1, "workspace")):
         refused("hb_linear_xent_backward", put(ok, at, v), what)
