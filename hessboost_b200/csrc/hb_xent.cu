@@ -139,11 +139,17 @@ struct Operand {
 struct Sizes {
   uint64_t n_rows, n_classes;
   uint32_t width, padded;
-  int planes;
+  int planes, g_planes;
 };
 
+// Up to this many rows a bf16 layer's G is kept in two pieces: its rounding
+// makes dx and dw 1.41 times one rounding off on average, but more over few
+// rows, and over few rows the weights' bytes take longer than the products.
+constexpr uint64_t kExactRows = 256;
+
 Sizes sizes_of(int32_t dtype, uint64_t n_rows, uint32_t width, uint64_t n_classes) {
-  return {n_rows, n_classes, width, (uint32_t)round_up(width, 64), dtype == HB_F32 ? 3 : 1};
+  return {n_rows, n_classes, width, (uint32_t)round_up(width, 64), dtype == HB_F32 ? 3 : 1,
+          dtype == HB_F32 ? 3 : n_rows <= kExactRows ? 2 : 1};
 }
 // bf16 rows of whole 64-column blocks are read as they lie where the address
 // and the row stride are whole 16-byte units, as TMA wants them.
@@ -178,13 +184,13 @@ int last_cols(uint64_t cols, int n, bool pair) {
   return n;
 }
 // Parts of k: enough tiles for the workers, at least 4 steps of 64 each. In
-// f32 a part is at most 2,048 long: the tensor cores' own sums round towards
+// f32 a part is at most 1,024 long: the tensor cores' own sums round towards
 // zero, and over 4,099 rows that was 2e-6 of dw, twice what f32 sums that
 // round to nearest are off.
 int k_splits(uint64_t tiles, int k_blocks, int workers, int planes) {
   const int want = tiles >= (uint64_t)workers ? 1 : (int)((workers + tiles - 1) / tiles);
   const int by_tiles = std::max(1, std::min(want, k_blocks * kMmaDepth / 4));
-  return planes == 1 ? by_tiles : std::max(by_tiles, std::min(32, (k_blocks * kMmaDepth * 64 + 2047) / 2048));
+  return planes == 1 ? by_tiles : std::max(by_tiles, std::min(32, (k_blocks * kMmaDepth * 64 + 1023) / 1024));
 }
 
 struct Forward {
@@ -224,7 +230,7 @@ Backward backward_plan(const Sizes& z, int32_t dtype, const void* x, uint64_t x_
   Backward b;
   b.x = operand_of(z, dtype, x, x_stride, z.n_rows, true);
   b.w = operand_of(z, dtype, w, w_stride, z.n_classes, false);
-  const uint64_t most = (uint64_t)kGradElements / z.planes;
+  const uint64_t most = (uint64_t)kGradElements / z.g_planes;
   const uint64_t least = 2048;  // classes of a piece, where there are as many
   b.chunk = std::min(z.n_rows, std::max<uint64_t>(most / std::min(z.n_classes, least) / 256 * 256, 256));
   b.chunks = (z.n_rows + b.chunk - 1) / b.chunk;
@@ -247,7 +253,7 @@ Backward backward_plan(const Sizes& z, int32_t dtype, const void* x, uint64_t x_
   b.dw_acc = b.dw_splits > 1 || b.chunks > 1;
   b.acc_stride = (uint32_t)round_up(z.width, 4);
   b.dw_rows = b.chunks > 1 ? z.n_classes : b.piece;
-  b.g_bytes = round_up(2ull * z.planes * b.chunk * b.g_stride, 256);
+  b.g_bytes = round_up(2ull * z.g_planes * b.chunk * b.g_stride, 256);
   b.dx_bytes = b.dx_acc ? round_up(4ull * b.dx_splits * b.chunk * b.acc_stride, 256) : 0;
   b.dw_bytes = b.dw_acc ? round_up(4ull * b.dw_splits * b.dw_rows * b.acc_stride, 256) : 0;
   b.bytes = b.x.bytes + b.w.bytes + (b.pieces * b.chunks > 1 ? 2 : 1) * b.g_bytes + b.dx_bytes + b.dw_bytes;
@@ -361,6 +367,7 @@ hb_status hb_linear_xent_forward(int32_t device, const void* x, uint64_t x_strid
   p.part = (float2*)at;
   p.at_label = (float*)(at + f.part);
   p.planes = z.planes;
+  p.g_planes = z.g_planes;
   p.all_classes = (int64_t)n_classes;
   p.width = (int)width;
   p.labels = labels;
@@ -447,6 +454,7 @@ hb_status hb_linear_xent_backward(int32_t device, const float* dloss, uint64_t d
   float* dx_acc = (float*)at;
   float* dw_acc = (float*)(at + b.dx_bytes);
   p.planes = z.planes;
+  p.g_planes = z.g_planes;
   p.all_classes = (int64_t)n_classes;
   p.width = (int)width;
   p.labels = labels;
@@ -477,7 +485,7 @@ hb_status hb_linear_xent_backward(int32_t device, const float* dloss, uint64_t d
       job.class0 = (int)v0, job.n_classes = (int)std::min(b.piece, n_classes - v0);
     };
     const auto g_lay = [&](const MmaJob& job, uint64_t step) {
-      return Lay{g[step & 1], (uint64_t)job.n_rows, b.g_stride, b.chunk * b.g_stride, z.planes, (job.n_classes + 63) / 64};
+      return Lay{g[step & 1], (uint64_t)job.n_rows, b.g_stride, b.chunk * b.g_stride, z.g_planes, (job.n_classes + 63) / 64};
     };
     MmaJob done{};
     void *dx_to = nullptr, *dw_to = nullptr;

@@ -44,7 +44,7 @@ struct MmaParams {
   CUtensorMap g_out;           // what grad writes (dx and dw read an earlier launch's)
   MmaJob jobs[kMaxJobs];
   int n_jobs;
-  int planes;                  // 1: bf16; 3: f32 in three pieces
+  int planes, g_planes;        // of x and w 1: bf16; 3: f32 in three pieces; G's: 1 to 3
   int width;
   const void* labels;          // of the call's rows, as the next three
   int label_type;

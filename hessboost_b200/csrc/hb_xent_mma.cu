@@ -52,9 +52,9 @@ struct Shape {
 constexpr float kLog2e = 1.4426950408889634f;
 
 // (piece of A, piece of B) of the products, smallest first; the last one
-// alone for bf16 operands.
-__constant__ int kPairA[6] = {2, 0, 1, 1, 0, 0};
-__constant__ int kPairB[6] = {0, 2, 1, 0, 1, 0};
+// alone for bf16 operands, the last two where G is in two pieces.
+__constant__ int kPairA[6] = {2, 0, 1, 0, 1, 0};
+__constant__ int kPairB[6] = {0, 2, 1, 1, 0, 0};
 
 // The mantissa, in [1, 2), of the first row's factor: G is formed in units
 // of it and dx and dw multiplied by it again in f32. A factor that is the
@@ -137,7 +137,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_xent_mma(const __grid_constant_
   const auto acc_empty = [&](int b) { return bars + 8u * (2 * kStages + 2 + b); };
   __shared__ uint32_t s_tmem;
   __shared__ volatile uint32_t s_gave_up;
-  constexpr int kPairs = kSplit ? 6 : 1;
+  const auto pairs_of = [&](const MmaJob& job) { return kSplit ? 6 : job.kind == kJobDx || job.kind == kJobDw ? p.g_planes : 1; };
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = kPair ? blockIdx.x & 1 : 0, worker = blockIdx.x / S::kCtas;
   if (threadIdx.x == 0) {
@@ -169,7 +169,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_xent_mma(const __grid_constant_
       const int a_row = (at.m * S::kCtas + rank) * 128 + (ma == &p.x_k ? job.row0 : 0);
       const int b_row = at.n * job.n_size + rank * share + (mb == &p.w_k ? job.class0 : 0);
       const int bk0 = mb == &p.w_mn ? job.class0 : mb == &p.x_mn ? job.row0 : 0;
-      for (int q = 6 - kPairs; q < 6; ++q) {
+      for (int q = 6 - pairs_of(job); q < 6; ++q) {
         const int pa = kPairA[q], pb = kPairB[q];
         for (int k = at.k0; k < at.k1; ++k) {
           if (!(ok = bar_wait(empty(r.stage), r.parity ^ 1u, &s_gave_up))) return false;
@@ -212,7 +212,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_xent_mma(const __grid_constant_
       // rows on; mn-major: 16 of k are 16 rows of 128 bytes on
       const uint32_t share = job.n_size / S::kCtas;  // k-major tiles are all alike
       const uint32_t block_a = a_mn ? 64 * kRow >> 4 : 128 * kRow >> 4, block_b = b_mn ? 64 * kRow >> 4 : share * kRow >> 4;
-      for (int q = 0; q < kPairs; ++q)
+      for (int q = pairs_of(job); q > 0; --q)
         for (int k = at.k0; k < at.k1; ++k) {
           if (!bar_wait(full(r.stage), r.parity, &s_gave_up)) return false;
           fence_after();
@@ -296,9 +296,13 @@ __global__ void __launch_bounds__(kThreads, 1) k_xent_mma(const __grid_constant_
         const int64_t rel = label - job.class0 - col0;
         // a row without a label: logits and lse 0 (its operand row is 0), factor 0
         const float each = !ok ? NAN : label >= 0 ? p.dloss[(size_t)(job.row0 + row) * p.dloss_stride] / unit_of<kSplit>(p) : 0.0f;
-        // lse log2(e) as a rounded value and, for f32, what the rounding left
-        const float l = label >= 0 ? p.lse[job.row0 + row] : 0.0f;
-        const float hi = l * kLog2e, lo = kSplit ? fmaf(l, kLog2e, -hi) : 0.0f;
+        // exp(z - lse) = 2^(z log2(e) - lse log2(e)). For f32, whose rounding of
+        // that difference (about -13 here and there) would be 3e-7 of the
+        // result: lse log2(e) = hi + lo with hi a multiple of 2^-9, whole parts
+        // taken out exactly, 2^x of what is left
+        const float l = label >= 0 ? p.lse[job.row0 + row] : 0.0f, product = l * kLog2e;
+        const float hi = kSplit ? rintf(product * 512.0f) * (1.0f / 512.0f) : product;
+        const float lo = kSplit ? fmaf(l, kLog2e, -hi) : 0.0f;
         for (int c = c0; c < c1; c += 64) {
           const int left = job.n_classes - (col0 + c);
           if (left <= 0) break;  // nothing of G there
@@ -307,9 +311,13 @@ __global__ void __launch_bounds__(kThreads, 1) k_xent_mma(const __grid_constant_
           tmem_load32(acc + c + 32, reinterpret_cast<float(&)[32]>(v[32]));
 #pragma unroll
           for (int i = 0; i < 64; ++i) {
-            float g = fmaf(v[i], kLog2e, -hi);
-            if (kSplit) g -= lo;
-            v[i] = exp2_fast(g);
+            const float g = fmaf(v[i], kLog2e, -hi);
+            if (kSplit) {
+              const float whole = fminf(fmaxf(rintf(g), -126.0f), 127.0f);
+              v[i] = exp2_fast(fmaf(v[i], kLog2e, -(hi + whole)) - lo) * __int_as_float(((int)whole + 127) << 23);
+            } else {
+              v[i] = exp2_fast(g);
+            }
           }
           if (rel >= c && rel < c + 64) {
             const int hit = (int)rel - c;
@@ -322,8 +330,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_xent_mma(const __grid_constant_
 #pragma unroll
             for (int i = 0; i < 64; ++i) v[i] = i < left ? v[i] : 0.0f;
           }
-#pragma unroll
-          for (int q = 0; q < (kSplit ? 3 : 1); ++q) {
+#pragma unroll 1
+          for (int q = 0; q < p.g_planes; ++q) {
             if (lane == 0) tma_wait_read<0>();
             __syncwarp();
 #pragma unroll
@@ -333,7 +341,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_xent_mma(const __grid_constant_
               for (int j = 0; j < 4; ++j) {
                 const __nv_bfloat162 b = __floats2bfloat162_rn(v[8 * i + 2 * j], v[8 * i + 2 * j + 1]);
                 h[j] = *reinterpret_cast<const uint32_t*>(&b);
-                if (kSplit) {
+                if (kSplit || p.g_planes > 1) {
                   v[8 * i + 2 * j] -= __low2float(b);
                   v[8 * i + 2 * j + 1] -= __high2float(b);
                 }

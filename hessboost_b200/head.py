@@ -16,6 +16,7 @@ argument raises ValueError before anything runs, a call that the library
 refuses raises HbError. Results do not change from run to run.
 """
 
+import array
 import ctypes
 import operator
 
@@ -281,38 +282,37 @@ def linear_xent_backward(dloss, x, weight, labels, lse):
 
 
 # -------------------------------------------------------------- clipping
-_of = operator.attrgetter
-_contiguous = operator.methodcaller("is_contiguous")
-_data_ptr = operator.methodcaller("data_ptr")
-_numel = operator.methodcaller("numel")
+_dtype = operator.attrgetter("dtype")
+_Tensor = torch.Tensor
 
 
 def _tensor_list(tensors):
-    """The host arrays of a list of contiguous tensors on one device, and that device. (Hundreds of tensors: each
-    question is asked of all of them in one call.)"""
-    n = len(tensors)
-    _need(n > 0, "tensors is empty")
-    devices = set(map(_of("device"), tensors))
+    """(n, addresses, elements, type codes, device) of a list of contiguous tensors on one device, the middle three as
+    host arrays. (Hundreds of tensors: each question is asked of all of them in one call.)"""
+    _need(len(tensors) > 0, "tensors is empty")
+    devices = set(map(_Tensor.get_device, tensors))
+    _need(devices != {-1}, "tensors must be on a CUDA device")
     _need(len(devices) == 1, "tensors must be on one device")
-    device = devices.pop()
-    _need(device.type == "cuda", "tensors must be on a CUDA device")
-    _need(all(map(_contiguous, tensors)), "tensors must be contiguous")
-    dtypes = list(map(_of("dtype"), tensors))
+    _need(all(map(_Tensor.is_contiguous, tensors)), "tensors must be contiguous")
+    dtypes = list(map(_dtype, tensors))
     _need(_TYPES.keys() >= set(dtypes), "tensors must be float32, float16 or bfloat16")
-    sizes = list(map(_numel, tensors))
-    return (n, (ctypes.c_void_p * n)(*map(_data_ptr, tensors)), (ctypes.c_uint64 * n)(*sizes),
-            (ctypes.c_int32 * n)(*map(_TYPES.__getitem__, dtypes)), device.index, sizes, dtypes)
+    return (len(tensors), array.array("Q", map(_Tensor.data_ptr, tensors)), array.array("Q", map(_Tensor.numel, tensors)),
+            array.array("i", map(_TYPES.__getitem__, dtypes)), devices.pop())
+
+
+def _address(a):
+    return a.buffer_info()[0]
 
 
 def grad_norm(tensors):
     """The 2-norm of all the tensors' elements together, a float32 scalar tensor on their device."""
     tensors = list(tensors)
-    n, ptrs, sizes, types, dev, _, _ = _tensor_list(tensors)
+    n, ptrs, sizes, types, dev = _tensor_list(tensors)
     L = lib()
     norm = torch.empty((), dtype=torch.float32, device=tensors[0].device)
     ws, size = _workspace(L.hb_grad_norm_workspace, norm.device, dev, n)
-    _check(L.hb_grad_norm(dev, n, ptrs, sizes, types, norm.data_ptr(), ws.data_ptr(), size, _stream(dev)),
-           "hb_grad_norm")
+    _check(L.hb_grad_norm(dev, n, _address(ptrs), _address(sizes), _address(types), norm.data_ptr(), ws.data_ptr(),
+                          size, _stream(dev)), "hb_grad_norm")
     return norm
 
 
@@ -322,20 +322,19 @@ def clip_grad_norm(tensors, max_norm, *, out=None):
     the results through that factor."""
     tensors = list(tensors)
     _need(max_norm >= 0, "max_norm must be >= 0")
-    n, ptrs, sizes, types, dev, numels, dtypes = _tensor_list(tensors)
+    n, ptrs, sizes, types, dev = _tensor_list(tensors)
     outs = ptrs
     if out is not None:
         out = list(out)
         _need(len(out) == n, "out must have a tensor for each of tensors")
-        _need(set(map(_of("device"), out)) == {tensors[0].device}, "tensors must be on one device")
-        _need(list(map(_numel, out)) == numels and list(map(_of("dtype"), out)) == dtypes and all(map(_contiguous, out)),
-              "out must be contiguous tensors of the same sizes and types")
-        outs = (ctypes.c_void_p * n)(*map(_data_ptr, out))
+        _, outs, out_sizes, out_types, out_dev = _tensor_list(out)
+        _need(out_dev == dev and out_sizes == sizes and out_types == types,
+              "out must be tensors of the same sizes and types on the same device")
     L = lib()
     norm = torch.empty((), dtype=torch.float32, device=tensors[0].device)
     ws, size = _workspace(L.hb_grad_norm_workspace, norm.device, dev, n)
-    _check(L.hb_clip_grad_norm(dev, n, ptrs, outs, sizes, types, max_norm, norm.data_ptr(), ws.data_ptr(), size,
-                               _stream(dev)), "hb_clip_grad_norm")
+    _check(L.hb_clip_grad_norm(dev, n, _address(ptrs), _address(outs), _address(sizes), _address(types), max_norm,
+                               norm.data_ptr(), ws.data_ptr(), size, _stream(dev)), "hb_clip_grad_norm")
     return norm
 
 
