@@ -347,7 +347,7 @@ hb_status hb_linear_xent_forward(int32_t device, const void* x, uint64_t x_strid
   if (few_applies(dtype, width, n_classes)) {
     DeviceScope dev(device);
     if (!dev.ok()) return fail(HB_REFUSED, "no such device");
-    few_forward(XentCall{x, w, labels, x_stride, w_stride, n_rows, n_classes, width, label_type}, loss, lse, device, sms,
+    few_forward(XentCall{x, w, labels, x_stride, w_stride, n_rows, n_classes, width, label_type}, loss, lse, sms,
                 (cudaStream_t)stream);
     return launched("hb_linear_xent_forward");
   }
@@ -423,7 +423,7 @@ hb_status hb_linear_xent_backward(int32_t device, const float* dloss, uint64_t d
     DeviceScope dev(device);
     if (!dev.ok()) return fail(HB_REFUSED, "no such device");
     few_backward(XentCall{x, w, labels, x_stride, w_stride, n_rows, n_classes, width, label_type}, dloss, dloss_stride, lse, dx, dw,
-                 workspace, device, sms, (cudaStream_t)stream);
+                 workspace, sms, (cudaStream_t)stream);
     return launched("hb_linear_xent_backward");
   }
   Backward b{};

@@ -87,9 +87,9 @@ struct XentCall {
 bool few_applies(int32_t dtype, uint32_t width, uint64_t n_classes);
 // Workspace of the backward call.
 uint64_t few_bytes(uint64_t n_rows, uint32_t width, uint64_t n_classes, int sms);
-void few_forward(const XentCall& c, float* loss, float* lse, int device, int sms, cudaStream_t s);
+void few_forward(const XentCall& c, float* loss, float* lse, int sms, cudaStream_t s);
 void few_backward(const XentCall& c, const float* dloss, uint64_t dloss_stride, const float* lse, void* dx, void* dw, void* workspace,
-                  int device, int sms, cudaStream_t s);
+                  int sms, cudaStream_t s);
 
 }  // namespace head
 }  // namespace hb

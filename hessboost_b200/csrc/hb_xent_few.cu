@@ -1,21 +1,23 @@
-// Linear softmax cross entropy over a few classes in f32, where the logits of
-// a row fit a thread's registers: x is read once forward and once backward,
-// without the three-piece products (hb_xent_mma.cu) that f32 takes there.
+// Linear softmax cross entropy over a few classes in f32: x is read once
+// forward and once backward, without the three-piece products
+// (hb_xent_mma.cu) that f32 takes there.
 //
-// A CTA keeps the weights in shared memory, [column][class]; a thread has one
-// row of a tile of 128. x comes in pieces of 32 columns by asynchronous
-// copies into a ring of kHeld pieces, all of them at once where the width
-// allows; backward then takes x from there again. A thread turns its logits
-// into its row of G; for each piece a warp sums dw over its 32 rows in order
-// and the warps' sums are added in order to the CTA's, and each thread forms
-// its row's piece of dx in x's place. The CTAs' sums of dw are added in order
-// at the end.
+// A warp keeps the weights in registers, a lane those of columns lane, lane +
+// 32, ... and takes a few rows at a time, as many as make 32 logits. Each lane
+// forms its columns' share of every logit; the shares are summed over the
+// lanes so that lane l ends up with logit l (31 exchanges for the 32), and the
+// softmax of a row is a few more between its lanes. Backward, the lanes hand
+// their element of G round, and every lane forms dx of its columns and adds to
+// its columns' part of dw, also in registers. The warps' parts of dw are
+// added in order, then the CTAs'.
 //
-// Bound by the broadcast reads of the weights (a 16-byte one for four products
-// of a row): 131,072 x 100 rows and 10 classes take 43 us forward and 102 us
-// backward, where x's bytes alone would take 8 and 16.
+// Bound by issuing and by the exchanges' latency: of 131,072 x 100 rows with
+// 10 classes x's bytes alone would take 8 us forward and 16 us backward; they
+// take 39 and 60. With the weights in shared memory and a thread a row, the
+// reads of them took 43 and 102 us, the tensor cores' pieces 87 and 250.
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "hb_xent.h"
 
@@ -23,12 +25,8 @@ namespace hb {
 namespace head {
 namespace {
 
-constexpr int kFewThreads = 128;        // and rows of a tile
+constexpr int kFewThreads = 128;
 constexpr int kWarps = kFewThreads / 32;
-constexpr int kPiece = 32;              // columns of a piece
-constexpr int kHeld = 4;                // pieces in shared memory
-constexpr int kRowStride = kPiece + 1;  // of a piece's row
-constexpr uint32_t kPieceFloats = kFewThreads * kRowStride;
 
 struct FewParams {
   const float *x, *w;
@@ -47,64 +45,11 @@ struct FewParams {
   }
 };
 
-__host__ __device__ constexpr uint32_t pieces_of(uint32_t width) { return (width + kPiece - 1) / kPiece; }
-// Floats of shared memory: the weights, the pieces, and backward dw's sums,
-// the warps' parts of them and G.
+// kClasses (a multiple of 4) classes over kLanes lanes, kRows rows at a time.
 template <int kClasses>
 struct Few {
-  static constexpr int kGStride = kClasses + 4;  // whole 16-byte units
-  static uint32_t weights(uint32_t width) { return pieces_of(width) * kPiece * kClasses; }
-  static uint32_t held(uint32_t width) { return std::min<uint32_t>(kHeld, pieces_of(width)) * kPieceFloats; }
-  static uint32_t forward_bytes(uint32_t width) { return 4 * (weights(width) + held(width)); }
-  static uint32_t backward_bytes(uint32_t width) {
-    return forward_bytes(width) + 4 * (weights(width) + kWarps * kPiece * kClasses + kFewThreads * kGStride);
-  }
-};
-
-// The weights, [column][class], zeros past either's end.
-template <int kClasses>
-__device__ __forceinline__ void load_weights(const FewParams& p, float* s_w) {
-  const uint32_t columns = pieces_of(p.width) * kPiece;
-  for (uint32_t i = threadIdx.x; i < columns * kClasses; i += kFewThreads) {
-    const uint32_t v = i / columns, d = i - v * columns;
-    s_w[d * kClasses + v] = v < (uint32_t)p.n_classes && d < p.width ? p.w[v * p.w_stride + d] : 0.0f;
-  }
-}
-
-// The ring of a tile's pieces: load k is of piece k mod pieces, into place k
-// mod kHeld; `loads` of them in all.
-struct Pieces {
-  float* s_x;
-  uint32_t pieces, loads;
-  __device__ __forceinline__ float* at(uint32_t k) const { return s_x + k % kHeld * kPieceFloats; }
-  // Starts load k, a warp a row at a time (zeros past either end), or nothing.
-  __device__ __forceinline__ void load(const FewParams& p, uint64_t row0, uint32_t k) const {
-    if (k < loads) {
-      const int lane = threadIdx.x & 31;
-      const uint32_t d = k % pieces * kPiece + lane;
-      const uint32_t rows = (uint32_t)min((uint64_t)kFewThreads, p.n_rows - row0);
-      const float* from = p.x + row0 * p.x_stride + d;
-      float* to = at(k) + lane;
-#pragma unroll 8
-      for (uint32_t r = threadIdx.x >> 5; r < kFewThreads; r += kWarps) {
-        if (r < rows && d < p.width)
-          asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"((uint32_t)__cvta_generic_to_shared(to + r * kRowStride)),
-                       "l"(from + r * p.x_stride)
-                       : "memory");
-        else
-          to[r * kRowStride] = 0.0f;
-      }
-    }
-    asm volatile("cp.async.commit_group;" ::: "memory");
-  }
-  __device__ __forceinline__ void begin(const FewParams& p, uint64_t row0) const {
-    for (uint32_t k = 0; k < kHeld; ++k) load(p, row0, k);
-  }
-  // The oldest load but kHeld - 1 has landed, for every thread.
-  __device__ __forceinline__ void wait() const {
-    asm volatile("cp.async.wait_group %0;" ::"n"(kHeld - 1) : "memory");
-    __syncthreads();
-  }
+  static constexpr int kLanes = kClasses <= 4 ? 4 : kClasses <= 8 ? 8 : kClasses <= 16 ? 16 : 32;
+  static constexpr int kRows = 32 / kLanes;
 };
 
 __device__ __forceinline__ void fma2(float& a0, float& a1, float b0, float b1, float c) {
@@ -115,169 +60,156 @@ __device__ __forceinline__ void fma2(float& a0, float& a1, float b0, float b1, f
   a0 = a.x, a1 = a.y;
 }
 
-// The logits of the thread's row; load k is used and load k + kHeld started.
-template <int kClasses>
-__device__ __forceinline__ void logits(const FewParams& p, const float* s_w, const Pieces& x, uint64_t row0, float (&z)[kClasses]) {
+// The lane's columns lane + 32 j of the weights.
+template <int kClasses, int J>
+__device__ __forceinline__ void load_weights(const FewParams& p, float (&w)[J][kClasses]) {
+  const uint32_t lane = threadIdx.x & 31;
 #pragma unroll
-  for (int v = 0; v < kClasses; ++v) z[v] = 0.0f;
-  for (uint32_t k = 0; k < x.pieces; ++k) {
-    x.wait();
-    const float* mine = x.at(k) + threadIdx.x * kRowStride;
-    const float4* w = reinterpret_cast<const float4*>(s_w + k * kPiece * kClasses);
-#pragma unroll 8
-    for (int d = 0; d < kPiece; ++d) {
-      const float a = mine[d];
+  for (int j = 0; j < J; ++j)
 #pragma unroll
-      for (int v = 0; v < kClasses / 4; ++v) {
-        const float4 q = w[d * (kClasses / 4) + v];
-        fma2(z[4 * v], z[4 * v + 1], q.x, q.y, a);
-        fma2(z[4 * v + 2], z[4 * v + 3], q.z, q.w, a);
-      }
-    }
-    if (k + kHeld < x.loads) __syncthreads();
-    x.load(p, row0, k + kHeld);
-  }
+    for (int v = 0; v < kClasses; ++v)
+      w[j][v] = lane + 32 * j < p.width && v < p.n_classes ? p.w[v * p.w_stride + lane + 32 * j] : 0.0f;
 }
 
-template <int kClasses>
-__global__ void __launch_bounds__(kFewThreads) k_few_forward(const FewParams p) {
-  extern __shared__ __align__(16) float sm[];
-  const uint32_t pieces = pieces_of(p.width);
-  float* s_w = sm;
-  const Pieces x{s_w + pieces * kPiece * kClasses, pieces, pieces};
-  uint64_t row0 = (uint64_t)blockIdx.x * kFewThreads;
-  x.begin(p, row0);
-  load_weights<kClasses>(p, s_w);
-  while (true) {
-    const uint64_t r = row0 + threadIdx.x, next = row0 + (uint64_t)gridDim.x * kFewThreads;
-    const int label = r < p.n_rows ? p.label(r) : -1;
-    float z[kClasses];
-    logits<kClasses>(p, s_w, x, row0, z);
-    if (next < p.n_rows) {
-      __syncthreads();
-      x.begin(p, next);
+// The lane's columns of the rows row0 + k, zeros where there are none.
+template <int kRows, int J>
+__device__ __forceinline__ void load_rows(const FewParams& p, uint64_t row0, float (&x)[kRows][J]) {
+  const uint32_t lane = threadIdx.x & 31;
+  const float* from = p.x + row0 * p.x_stride + lane;
+#pragma unroll
+  for (int k = 0; k < kRows; ++k)
+#pragma unroll
+    for (int j = 0; j < J; ++j) x[k][j] = row0 + k < p.n_rows && lane + 32 * j < p.width ? from[k * p.x_stride + 32 * j] : 0.0f;
+}
+
+// Logit (row l / kLanes, class l mod kLanes) of the warp's rows, in lane l.
+template <int kClasses, int J>
+__device__ __forceinline__ float logits(const float (&w)[J][kClasses], const float (&x)[Few<kClasses>::kRows][J]) {
+  using F = Few<kClasses>;
+  const int lane = threadIdx.x & 31;
+  float a[32];
+#pragma unroll
+  for (int i = 0; i < 32; ++i) a[i] = 0.0f;
+#pragma unroll
+  for (int k = 0; k < F::kRows; ++k)
+#pragma unroll
+    for (int j = 0; j < J; ++j)
+#pragma unroll
+      for (int v = 0; v < kClasses; v += 2) fma2(a[k * F::kLanes + v], a[k * F::kLanes + v + 1], w[j][v], w[j][v + 1], x[k][j]);
+  // lane l keeps the half of the values that l's bit names, and gets the
+  // other lane's share of it
+#pragma unroll
+  for (int s = 16; s; s >>= 1)
+#pragma unroll
+    for (int i = 0; i < s; ++i) {
+      const bool up = lane & s;
+      const float keep = up ? a[i + s] : a[i], give = up ? a[i] : a[i + s];
+      a[i] = keep + __shfl_xor_sync(0xffffffffu, give, s);
     }
-    if (r < p.n_rows) {
-      float top = -INFINITY, at = 0.0f, s = 0.0f;
+  return a[0];
+}
+
+template <int kClasses, int J>
+__global__ void __launch_bounds__(kFewThreads) k_few_forward(const FewParams p) {
+  using F = Few<kClasses>;
+  const int lane = threadIdx.x & 31, v = lane % F::kLanes, k = lane / F::kLanes;
+  float w[J][kClasses], x[F::kRows][J], next[F::kRows][J];
+  load_weights(p, w);
+  const uint64_t step = (uint64_t)gridDim.x * kWarps * F::kRows;
+  uint64_t row0 = ((uint64_t)blockIdx.x * kWarps + (threadIdx.x >> 5)) * F::kRows;
+  load_rows(p, row0, next);
+  for (; row0 < p.n_rows; row0 += step) {
 #pragma unroll
-      for (int v = 0; v < kClasses; ++v) {
-        if (v < p.n_classes) top = fmaxf(top, z[v]);
-        if (v == label) at = z[v];
-      }
-      const float from = top == -INFINITY ? 0.0f : top;
+    for (int i = 0; i < F::kRows; ++i)
 #pragma unroll
-      for (int v = 0; v < kClasses; ++v)
-        if (v < p.n_classes) s += expf(z[v] - from);
-      const float lse = from + logf(s);
+      for (int j = 0; j < J; ++j) x[i][j] = next[i][j];
+    const uint64_t r = row0 + k;
+    const bool in = r < p.n_rows;
+    const int label = in ? p.label(r) : -1;
+    load_rows(p, row0 + step, next);
+    const float z = logits(w, x);
+    const bool there = v < p.n_classes;
+    float top = there ? z : -INFINITY;
+#pragma unroll
+    for (int s = F::kLanes / 2; s; s >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, s));
+    const float from = top == -INFINITY ? 0.0f : top;
+    float sum = there ? expf(z - from) : 0.0f;
+#pragma unroll
+    for (int s = F::kLanes / 2; s; s >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
+    const float at = __shfl_sync(0xffffffffu, z, k * F::kLanes + max(label, 0));
+    if (v == 0 && in) {
+      const float lse = from + logf(sum);
       p.lse[r] = lse;
       p.loss[r] = label >= 0 ? lse - at : 0.0f;
     }
-    if (next >= p.n_rows) break;
-    row0 = next;
   }
 }
 
-template <int kClasses>
+template <int kClasses, int J>
 __global__ void __launch_bounds__(kFewThreads) k_few_backward(const FewParams p) {
   using F = Few<kClasses>;
-  extern __shared__ __align__(16) float sm[];
-  const uint32_t pieces = pieces_of(p.width), weights = pieces * kPiece * kClasses;
-  float* s_w = sm;
-  float* s_dw = s_w + weights;                          // [column][class]
-  float* s_sum = s_dw + weights;                        // [warp][class][column of the piece]
-  float* s_g = s_sum + kWarps * kPiece * kClasses;      // [row][kGStride]
-  const bool held = pieces <= kHeld;                    // x stays for the second pass
-  const Pieces x{s_g + kFewThreads * F::kGStride, pieces, held ? pieces : 2 * pieces};
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  uint64_t row0 = (uint64_t)blockIdx.x * kFewThreads;
-  x.begin(p, row0);
-  load_weights<kClasses>(p, s_w);
-  for (uint32_t i = threadIdx.x; i < weights; i += kFewThreads) s_dw[i] = 0.0f;
-  while (true) {
-    const uint64_t r = row0 + threadIdx.x, next = row0 + (uint64_t)gridDim.x * kFewThreads;
+  extern __shared__ float s_dw[];  // [warp][class][32 J]
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, v = lane % F::kLanes, k = lane / F::kLanes;
+  float w[J][kClasses], dw[J][kClasses], x[F::kRows][J], next[F::kRows][J];
+  load_weights(p, w);
+#pragma unroll
+  for (int j = 0; j < J; ++j)
+#pragma unroll
+    for (int c = 0; c < kClasses; ++c) dw[j][c] = 0.0f;
+  const uint64_t step = (uint64_t)gridDim.x * kWarps * F::kRows;
+  uint64_t row0 = ((uint64_t)blockIdx.x * kWarps + warp) * F::kRows;
+  load_rows(p, row0, next);
+  for (; row0 < p.n_rows; row0 += step) {
+#pragma unroll
+    for (int i = 0; i < F::kRows; ++i)
+#pragma unroll
+      for (int j = 0; j < J; ++j) x[i][j] = next[i][j];
+    const uint64_t r = row0 + k;
     const int label = r < p.n_rows ? p.label(r) : -1;
     const float each = label >= 0 ? p.dloss[r * p.dloss_stride] : 0.0f, lse = label >= 0 ? p.lse[r] : 0.0f;
-    float g[kClasses];
-    logits<kClasses>(p, s_w, x, row0, g);
+    load_rows(p, row0 + step, next);
+    const float z = logits(w, x);
+    const float mine = label >= 0 && v < p.n_classes ? each * (expf(z - lse) - (v == label ? 1.0f : 0.0f)) : 0.0f;
 #pragma unroll
-    for (int v = 0; v < kClasses; ++v)
-      g[v] = label >= 0 && v < p.n_classes ? each * (expf(g[v] - lse) - (v == label ? 1.0f : 0.0f)) : 0.0f;
-#pragma unroll
-    for (int v = 0; v < kClasses; v += 4)
-      *reinterpret_cast<float4*>(s_g + threadIdx.x * F::kGStride + v) = make_float4(g[v], g[v + 1], g[v + 2], g[v + 3]);
-    for (uint32_t k = 0; k < pieces; ++k) {
-      const uint32_t load = held ? k : pieces + k;
-      if (!held) x.wait();
-      float* s_x = x.at(load);
+    for (int i = 0; i < F::kRows; ++i) {
       // a row without a label adds nothing to dw, whatever it holds
-      if (label < 0)
-        for (int d = 0; d < kPiece; ++d) s_x[threadIdx.x * kRowStride + d] = 0.0f;
-      __syncwarp();
-      // dw: column `lane` over the warp's rows (its own: their G is there too)
-      float acc[kClasses];
+      const bool labelled = __shfl_sync(0xffffffffu, label, i * F::kLanes) >= 0;
+      float g[kClasses];
 #pragma unroll
-      for (int v = 0; v < kClasses; ++v) acc[v] = 0.0f;
-#pragma unroll 4
-      for (int i = 0; i < 32; ++i) {
-        const float a = s_x[(warp * 32 + i) * kRowStride + lane];
-        const float4* gr = reinterpret_cast<const float4*>(s_g + (warp * 32 + i) * F::kGStride);
+      for (int c = 0; c < kClasses; ++c) g[c] = __shfl_sync(0xffffffffu, mine, i * F::kLanes + c);
+      float* out = p.dx + (row0 + i) * p.width + lane;
 #pragma unroll
-        for (int v = 0; v < kClasses / 4; ++v) {
-          const float4 q = gr[v];
-          fma2(acc[4 * v], acc[4 * v + 1], q.x, q.y, a);
-          fma2(acc[4 * v + 2], acc[4 * v + 3], q.z, q.w, a);
+      for (int j = 0; j < J; ++j) {
+        const float a = labelled ? x[i][j] : 0.0f;
+        float d = 0.0f, e = 0.0f;
+#pragma unroll
+        for (int c = 0; c < kClasses; c += 2) {
+          fma2(dw[j][c], dw[j][c + 1], g[c], g[c + 1], a);
+          d = fmaf(g[c], w[j][c], d), e = fmaf(g[c + 1], w[j][c + 1], e);
         }
+        if (row0 + i < p.n_rows && lane + 32 * j < p.width) out[32 * j] = d + e;
       }
-#pragma unroll
-      for (int v = 0; v < kClasses; ++v) s_sum[(warp * kClasses + v) * kPiece + lane] = acc[v];
-      __syncwarp();
-      // dx of the thread's row, in x's place
-      const float4* w = reinterpret_cast<const float4*>(s_w + k * kPiece * kClasses);
-#pragma unroll 8
-      for (int d = 0; d < kPiece; ++d) {
-        float a = 0.0f, b = 0.0f;
-#pragma unroll
-        for (int v = 0; v < kClasses / 4; ++v) {
-          const float4 q = w[d * (kClasses / 4) + v];
-          a = fmaf(g[4 * v], q.x, a), b = fmaf(g[4 * v + 1], q.y, b);
-          a = fmaf(g[4 * v + 2], q.z, a), b = fmaf(g[4 * v + 3], q.w, b);
-        }
-        s_x[threadIdx.x * kRowStride + d] = a + b;
-      }
-      __syncthreads();
-      for (int v = warp; v < kClasses; v += kWarps) {
-        float t = s_sum[v * kPiece + lane];
-#pragma unroll
-        for (int q = 1; q < kWarps; ++q) t += s_sum[(q * kClasses + v) * kPiece + lane];
-        s_dw[(k * kPiece + lane) * kClasses + v] += t;
-      }
-      const uint32_t d = k * kPiece + lane;
-      if (d < p.width) {
-        const uint32_t rows = (uint32_t)min((uint64_t)kFewThreads, p.n_rows - row0);
-        float* out = p.dx + row0 * p.width + d;
-#pragma unroll 8
-        for (uint32_t i = warp; i < rows; i += kWarps) out[(uint64_t)i * p.width] = s_x[i * kRowStride + lane];
-      }
-      __syncthreads();
-      if (!held) x.load(p, row0, load + kHeld);
     }
-    if (next >= p.n_rows) break;
-    row0 = next;
-    // (not held: the loads past the last were empty, as begin's first ones wait for nothing)
-    x.begin(p, row0);
   }
-  const uint32_t all = (uint32_t)p.n_classes * p.width;
-  for (uint32_t i = threadIdx.x; i < all; i += kFewThreads) {
-    const uint32_t v = i / p.width, d = i - v * p.width;
-    const float q = s_dw[d * kClasses + v];
-    if (gridDim.x == 1) p.dw[i] = q;
-    else p.part[(uint64_t)blockIdx.x * all + i] = q;
+#pragma unroll
+  for (int j = 0; j < J; ++j)
+#pragma unroll
+    for (int c = 0; c < kClasses; ++c) s_dw[(warp * kClasses + c) * (32 * J) + 32 * j + lane] = dw[j][c];
+  __syncthreads();
+  for (uint32_t i = threadIdx.x; i < (uint32_t)p.n_classes * (32 * J); i += kFewThreads) {
+    const uint32_t c = i / (32 * J), d = i % (32 * J);
+    if (d >= p.width) continue;
+    float t = s_dw[i];
+#pragma unroll
+    for (int q = 1; q < kWarps; ++q) t += s_dw[q * kClasses * (32 * J) + i];
+    if (gridDim.x == 1) p.dw[c * p.width + d] = t;
+    else p.part[((uint64_t)blockIdx.x * p.n_classes + c) * p.width + d] = t;
   }
 }
 
 // dw from the CTAs' sums: 32 elements a CTA, its warps each a share of the
 // sums in order, then the warps in order.
-constexpr int kJoinWarps = 8;
+constexpr int kJoinWarps = 16;
 __global__ void __launch_bounds__(32 * kJoinWarps) k_few_join(const float* __restrict__ part, int parts, uint32_t n, float* __restrict__ dw) {
   __shared__ float s[kJoinWarps][32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -294,66 +226,71 @@ __global__ void __launch_bounds__(32 * kJoinWarps) k_few_join(const float* __res
   dw[i] = a;
 }
 
-// f(padded number of classes) as a constant.
+// f(padded classes, columns a lane) as constants, where both fit a lane's
+// registers (64 weights); whether they do.
 template <typename F>
-void with_classes(int n, F&& f) {
+bool with_few(uint64_t n_classes, uint32_t width, F&& f) {
   using std::integral_constant;
-  if (n <= 4) f(integral_constant<int, 4>{});
-  else if (n <= 8) f(integral_constant<int, 8>{});
-  else if (n <= 12) f(integral_constant<int, 12>{});
-  else if (n <= 16) f(integral_constant<int, 16>{});
-  else if (n <= 24) f(integral_constant<int, 24>{});
-  else f(integral_constant<int, 32>{});
+  const auto columns = [&](auto c) {
+    constexpr int kMost = 64 / decltype(c)::value;
+    if (width <= 32) return f(c, integral_constant<int, 1>{}), true;
+    if (width <= 64) return f(c, integral_constant<int, 2>{}), true;
+    if constexpr (kMost >= 4)
+      if (width <= 128) return f(c, integral_constant<int, 4>{}), true;
+    if constexpr (kMost >= 8)
+      if (width <= 256) return f(c, integral_constant<int, 8>{}), true;
+    return false;
+  };
+  if (n_classes <= 4) return columns(integral_constant<int, 4>{});
+  if (n_classes <= 8) return columns(integral_constant<int, 8>{});
+  if (n_classes <= 12) return columns(integral_constant<int, 12>{});
+  if (n_classes <= 16) return columns(integral_constant<int, 16>{});
+  if (n_classes <= 24) return columns(integral_constant<int, 24>{});
+  if (n_classes <= 32) return columns(integral_constant<int, 32>{});
+  return false;
 }
 
-constexpr uint64_t kFewClasses = 32;
-constexpr uint64_t kFewWeights = 2048;       // padded classes x padded width
-constexpr uint64_t kPartBytes = 16ull << 20; // of the CTAs' sums of dw
-// CTAs: one a tile, or as many as leave no more than kPartBytes.
-uint64_t few_ctas(uint64_t n_rows, uint64_t n_classes, uint32_t width, int sms) {
-  const uint64_t most = std::max<uint64_t>(2 * sms, std::min<uint64_t>(16 * sms, kPartBytes / (4 * n_classes * width)));
-  return std::min((n_rows + kFewThreads - 1) / kFewThreads, most);
+// CTAs: at most as many as are there at once, about, by their registers.
+uint64_t few_ctas(uint64_t n_rows, uint64_t n_classes, uint32_t width, int sms, bool backward) {
+  uint64_t n = 0;
+  with_few(n_classes, width, [&](auto c, auto j) {
+    constexpr int kHeld = decltype(c)::value * decltype(j)::value;
+    const uint64_t rows = kWarps * Few<decltype(c)::value>::kRows;
+    const int regs = 60 + (backward ? 9 * kHeld / 4 : kHeld), fit = std::max(2, 512 / regs);
+    n = std::min<uint64_t>((n_rows + rows - 1) / rows, (uint64_t)fit * sms);
+  });
+  return n;
 }
 
 }  // namespace
 
-// f32 alone: bf16 products take one pass of the tensor cores, and 131,072 x
-// 64 rows with 16 classes take them 75 us backward, this 72. In f32 that is 72
-// us against 157; with 32 classes of 128 columns it is 273 against 212.
+// f32 alone: bf16 products take one pass of the tensor cores.
 bool few_applies(int32_t dtype, uint32_t width, uint64_t n_classes) {
-  if (dtype != HB_F32 || n_classes > kFewClasses) return false;
-  uint64_t weights = 0;
-  with_classes((int)n_classes, [&](auto c) { weights = (uint64_t)decltype(c)::value * pieces_of(width) * kPiece; });
-  return weights <= kFewWeights;
+  return dtype == HB_F32 && with_few(n_classes, width, [](auto, auto) {});
 }
 
 uint64_t few_bytes(uint64_t n_rows, uint32_t width, uint64_t n_classes, int sms) {
-  const uint64_t ctas = few_ctas(n_rows, n_classes, width, sms);
+  const uint64_t ctas = few_ctas(n_rows, n_classes, width, sms, true);
   return ctas > 1 ? 4 * ctas * n_classes * width : 0;
 }
 
-void few_forward(const XentCall& c, float* loss, float* lse, int device, int sms, cudaStream_t s) {
+void few_forward(const XentCall& c, float* loss, float* lse, int sms, cudaStream_t s) {
   const FewParams p{(const float*)c.x, (const float*)c.w, c.labels, c.x_stride, c.w_stride, c.n_rows, c.width, (int)c.n_classes, c.label_type,
                     loss, lse};
-  const unsigned ctas = (unsigned)few_ctas(c.n_rows, c.n_classes, c.width, sms);
-  with_classes(p.n_classes, [&](auto n) {
-    constexpr int kClasses = decltype(n)::value;
-    const uint32_t bytes = Few<kClasses>::forward_bytes(c.width);
-    allow_shared<k_few_forward<kClasses>>(device, bytes);
-    k_few_forward<kClasses><<<ctas, kFewThreads, bytes, s>>>(p);
+  const unsigned ctas = (unsigned)few_ctas(c.n_rows, c.n_classes, c.width, sms, false);
+  with_few(c.n_classes, c.width, [&](auto n, auto j) {
+    k_few_forward<decltype(n)::value, decltype(j)::value><<<ctas, kFewThreads, 0, s>>>(p);
   });
 }
 
 void few_backward(const XentCall& c, const float* dloss, uint64_t dloss_stride, const float* lse, void* dx, void* dw, void* workspace,
-                  int device, int sms, cudaStream_t s) {
+                  int sms, cudaStream_t s) {
   const FewParams p{(const float*)c.x, (const float*)c.w, c.labels, c.x_stride, c.w_stride, c.n_rows, c.width, (int)c.n_classes, c.label_type,
                     nullptr, const_cast<float*>(lse), dloss, dloss_stride, (float*)dx, (float*)dw, (float*)workspace};
-  const unsigned ctas = (unsigned)few_ctas(c.n_rows, c.n_classes, c.width, sms);
-  with_classes(p.n_classes, [&](auto n) {
-    constexpr int kClasses = decltype(n)::value;
-    const uint32_t bytes = Few<kClasses>::backward_bytes(c.width);
-    allow_shared<k_few_backward<kClasses>>(device, bytes);
-    k_few_backward<kClasses><<<ctas, kFewThreads, bytes, s>>>(p);
+  const unsigned ctas = (unsigned)few_ctas(c.n_rows, c.n_classes, c.width, sms, true);
+  with_few(c.n_classes, c.width, [&](auto n, auto j) {
+    constexpr int kClasses = decltype(n)::value, J = decltype(j)::value;
+    k_few_backward<kClasses, J><<<ctas, kFewThreads, 4 * kWarps * kClasses * 32 * J, s>>>(p);
   });
   const uint32_t all = (uint32_t)(c.n_classes * c.width);
   if (ctas > 1) k_few_join<<<(all + 31) / 32, 32 * kJoinWarps, 0, s>>>(p.part, (int)ctas, all, p.dw);
