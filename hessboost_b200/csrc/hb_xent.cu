@@ -168,12 +168,16 @@ int stages_of(uint64_t k) { return (int)((k + 64 * kMmaDepth - 1) / (64 * kMmaDe
 // Columns of a tile: as few whole tiles of at most 256 as there need be, all
 // alike (multiples of `unit`), or narrower ones where there are not enough
 // tiles for the workers.
-int tile_cols(uint64_t cols, uint64_t m_tiles, int workers, int unit) {
-  uint64_t n = (cols + 255) / 256;
+int tile_cols(uint64_t cols, uint64_t m_tiles, int workers, int unit, uint64_t most = 256) {
+  uint64_t n = (cols + most - 1) / most;
   while (m_tiles * n < (uint64_t)workers && (cols + n) / (n + 1) > 64) ++n;
   const auto size = [&](uint64_t k) { return round_up((cols + k - 1) / k, unit); };
   return (int)size(n);
 }
+// The most columns of a tile of logits: where k is summed in chunks, as many
+// as an epilogue warp can hold the sums of.
+uint64_t z_cols(const Sizes& z) { return z.planes > 1 && stages_of(z.width) > kXentChunk ? 128 : 256; }
+
 // Columns of the last of the tiles of n columns: 16 a CTA, 32, 64, or all,
 // where that is enough (each CTA's share then lies in whole blocks of 64, or
 // inside one).
@@ -205,7 +209,7 @@ Forward forward_plan(const Sizes& z, int32_t dtype, const void* x, uint64_t x_st
   f.w = operand_of(z, dtype, w, w_stride, z.n_classes, false);
   f.pair = use_pairs(z.n_rows, z.n_classes, z.width, sms);
   const int m = f.pair ? 256 : 128;
-  f.n_size = tile_cols(z.n_classes, (z.n_rows + m - 1) / m, f.pair ? sms / 2 : sms, f.pair ? 128 : 64);
+  f.n_size = tile_cols(z.n_classes, (z.n_rows + m - 1) / m, f.pair ? sms / 2 : sms, f.pair ? 128 : 64, z_cols(z));
   f.n_tiles = (int)((z.n_classes + f.n_size - 1) / f.n_size);
   f.chunk = std::min<uint64_t>(z.n_rows, std::max<uint64_t>(256, kPartBytes / (8ull * f.n_tiles) / 256 * 256));
   f.part = round_up(8ull * f.n_tiles * f.chunk, 256);
@@ -242,7 +246,7 @@ Backward backward_plan(const Sizes& z, int32_t dtype, const void* x, uint64_t x_
   const int m = b.pair ? 256 : 128, workers = b.pair ? sms / 2 : sms;
   b.g_stride = round_up(b.piece, 64);
   const uint64_t row_tiles = (b.chunk + m - 1) / m, class_tiles = (b.piece + m - 1) / m;
-  b.grad_n = tile_cols(b.piece, row_tiles, workers, b.pair ? 128 : 64);
+  b.grad_n = tile_cols(b.piece, row_tiles, workers, b.pair ? 128 : 64, z_cols(z));
   b.out_n = tile_cols(z.width, row_tiles + class_tiles, workers, b.pair ? 128 : 64);
   // two tiles of which one would be mostly empty: whole ones and a narrow last
   if (z.width > 256 && z.width % 256 <= 128) b.out_n = 256;

@@ -23,6 +23,7 @@ struct MmaOut {
 };
 
 constexpr int kMmaDepth = 2;  // blocks of 64 of k in a stage
+constexpr int kXentChunk = 4; // stages of z's k that f32 operands are summed over in the tensor cores
 
 // m_tiles x n_tiles tiles of (128 x CTAs) x n_size (the last ones n_last), k (k_total of it) in
 // k_blocks stages shared among `splits` tiles each; m_fast: consecutive tiles go down the rows.

@@ -23,7 +23,10 @@
 // f32 operands are three bf16 pieces (v = p0 + p1 + p2, each the rounding of
 // what the ones before leave), and a product is the six products of pieces
 // whose orders add up to at most 2: what is left out is below 2^-24 of the
-// operands' product. The smallest are summed first.
+// operands' product. The smallest are summed first. The tensor cores round
+// their sums towards zero, so a long k is summed in chunks of kChunk stages in
+// f32 arithmetic: z over 1,233 columns in one go left 8e-6 of the gradients
+// (for dx and dw, whose k is cut up anyway, see k_splits).
 #include <algorithm>
 #include <cmath>
 #include <string>
@@ -66,6 +69,13 @@ __device__ __forceinline__ float unit_of(const MmaParams& p) {
   const uint32_t bits = __float_as_uint(p.dloss[0]);
   const uint32_t e = bits >> 23 & 0xffu;
   return kSplit || e == 0u || e == 0xffu ? 1.0f : __uint_as_float((bits & 0x7fffffu) | 0x3f800000u);
+}
+
+// Stages of a chunk of z's k, and the chunks of a tile.
+constexpr int kChunk = kXentChunk;
+template <bool kSplit>
+__device__ __forceinline__ int chunks_of(const MmaJob& job, int k0, int k1) {
+  return kSplit && (job.kind == kJobStats || job.kind == kJobGrad) ? max(1, (k1 - k0 + kChunk - 1) / kChunk) : 1;
 }
 
 template <int kStages>
@@ -169,9 +179,11 @@ __global__ void __launch_bounds__(kThreads, 1) k_xent_mma(const __grid_constant_
       const int a_row = (at.m * S::kCtas + rank) * 128 + (ma == &p.x_k ? job.row0 : 0);
       const int b_row = at.n * job.n_size + rank * share + (mb == &p.w_k ? job.class0 : 0);
       const int bk0 = mb == &p.w_mn ? job.class0 : mb == &p.x_mn ? job.row0 : 0;
-      for (int q = 6 - pairs_of(job); q < 6; ++q) {
-        const int pa = kPairA[q], pb = kPairB[q];
-        for (int k = at.k0; k < at.k1; ++k) {
+      const int chunks = chunks_of<kSplit>(job, at.k0, at.k1), pairs = pairs_of(job);
+      for (int c = 0; c < chunks * pairs; ++c) {
+        const int q = 6 - pairs + c % pairs, pa = kPairA[q], pb = kPairB[q];
+        const int k0 = chunks > 1 ? at.k0 + c / pairs * kChunk : at.k0, k1 = chunks > 1 ? min(at.k1, k0 + kChunk) : at.k1;
+        for (int k = k0; k < k1; ++k) {
           if (!(ok = bar_wait(empty(r.stage), r.parity ^ 1u, &s_gave_up))) return false;
           const uint32_t dst = base + r.stage * S::kStageBytes;
           const uint32_t bar = kPair ? peer_addr(full(r.stage), 0) : full(r.stage);
@@ -203,17 +215,20 @@ __global__ void __launch_bounds__(kThreads, 1) k_xent_mma(const __grid_constant_
     each_tile(p, worker, [&](const MmaJob& job, const TileAt& at) {
       const bool a_mn = job.kind == kJobDw, b_mn = job.kind == kJobDx || job.kind == kJobDw;
       const uint32_t idesc = instr_desc(128 * S::kCtas, at.cols, a_mn, b_mn), sa = k_step(a_mn), sb = k_step(b_mn);
-      const int buf = tile & 1;
-      if (!bar_wait<kPair>(acc_empty(buf), ((tile >> 1) & 1) ^ 1, &s_gave_up)) return false;
-      fence_after();
-      const uint32_t d = tmem + buf * 256;
-      bool add = false;
       // k-major: 16 of k are 32 bytes on, the next block of 64 one block of
       // rows on; mn-major: 16 of k are 16 rows of 128 bytes on
       const uint32_t share = job.n_size / S::kCtas;  // k-major tiles are all alike
       const uint32_t block_a = a_mn ? 64 * kRow >> 4 : 128 * kRow >> 4, block_b = b_mn ? 64 * kRow >> 4 : share * kRow >> 4;
-      for (int q = pairs_of(job); q > 0; --q)
-        for (int k = at.k0; k < at.k1; ++k) {
+      const int chunks = chunks_of<kSplit>(job, at.k0, at.k1);
+      for (int c = 0; c < chunks; ++c, ++tile) {
+        const int buf = tile & 1;
+        if (!bar_wait<kPair>(acc_empty(buf), ((tile >> 1) & 1) ^ 1, &s_gave_up)) return false;
+        fence_after();
+        const uint32_t d = tmem + buf * 256;
+        bool add = false;
+        const int k0 = chunks > 1 ? at.k0 + c * kChunk : at.k0, k1 = chunks > 1 ? min(at.k1, k0 + kChunk) : at.k1;
+        for (int q = pairs_of(job); q > 0; --q)
+        for (int k = k0; k < k1; ++k) {
           if (!bar_wait(full(r.stage), r.parity, &s_gave_up)) return false;
           fence_after();
           const uint32_t dst = base + r.stage * S::kStageBytes;
@@ -228,8 +243,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_xent_mma(const __grid_constant_
           mma_commit<kPair>(empty(r.stage));
           r.next();
         }
-      mma_commit<kPair>(acc_full(buf));
-      ++tile;
+        mma_commit<kPair>(acc_full(buf));
+      }
       return true;
     });
   } else if (warp >= 4) {
@@ -240,14 +255,52 @@ __global__ void __launch_bounds__(kThreads, 1) k_xent_mma(const __grid_constant_
     const uint32_t stage = staging + (warp - 4) * 4096;
     int tile = 0;
     each_tile(p, worker, [&](const MmaJob& job, const TileAt& at) {
+      const int cut = min(at.cols, (at.cols / 2 + 63) & ~63), c0 = half ? cut : 0, c1 = half ? at.cols : cut;
+      const int chunks = chunks_of<kSplit>(job, at.k0, at.k1);
+      const auto release = [&](int buf) {
+        fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          if constexpr (kPair) bar_arrive_at(peer_addr(acc_empty(buf), 0)); else bar_arrive(acc_empty(buf));
+        }
+      };
+      // the chunks but the last, of the warp's 64 columns (tiles are 128 wide at most)
+      float sum[kSplit ? 64 : 1] = {};
+      bool ok = true;
+      if constexpr (kSplit) {
+        for (int c = 0; c + 1 < chunks; ++c, ++tile) {
+          const int buf = tile & 1;
+          ok = bar_wait(acc_full(buf), (tile >> 1) & 1, &s_gave_up) && ok;
+          __syncwarp();
+          fence_after();
+          if (c0 < c1) {
+            float v[32];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              tmem_load32(tmem + buf * 256 + ((uint32_t)(quarter * 32) << 16) + c0 + 32 * h, v);
+#pragma unroll
+              for (int i = 0; i < 32; ++i) sum[32 * h + i] += v[i];
+            }
+          }
+          release(buf);
+        }
+      }
       const int buf = tile & 1;
-      const bool ok = bar_wait(acc_full(buf), (tile >> 1) & 1, &s_gave_up);
+      ok = bar_wait(acc_full(buf), (tile >> 1) & 1, &s_gave_up) && ok;
       __syncwarp();
       fence_after();
       const uint32_t acc = tmem + buf * 256 + ((uint32_t)(quarter * 32) << 16);
+      // adds the chunks before to the accumulators of columns c and on
+      const auto add_chunks = [&](int c, float* v) {
+        if constexpr (kSplit) {
+          if (chunks > 1) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] += c == c0 ? sum[i] : sum[32 + i];
+          }
+        }
+      };
       const int row0 = (at.m * S::kCtas + rank) * 128 + quarter * 32, row = row0 + lane;
       const int col0 = at.n * job.n_size;
-      const int cut = min(at.cols, (at.cols / 2 + 63) & ~63), c0 = half ? cut : 0, c1 = half ? at.cols : cut;
       if (job.kind == kJobStats) {
         const bool in = row < job.n_rows;
         const int64_t rel = (in ? p.label((int64_t)job.row0 + row) : -1) - job.class0 - col0;
@@ -257,6 +310,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_xent_mma(const __grid_constant_
           if (left <= 0) break;
           float v[32];
           tmem_load32(acc + c, v);
+          add_chunks(c, v);
           if (left < 32) {
 #pragma unroll
             for (int i = 0; i < 32; ++i) v[i] = i < left ? v[i] : -INFINITY;
@@ -309,6 +363,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_xent_mma(const __grid_constant_
           float v[64];
           tmem_load32(acc + c, reinterpret_cast<float(&)[32]>(v[0]));
           tmem_load32(acc + c + 32, reinterpret_cast<float(&)[32]>(v[32]));
+          add_chunks(c, v);
+          add_chunks(c + 32, v + 32);
 #pragma unroll
           for (int i = 0; i < 64; ++i) {
             const float g = fmaf(v[i], kLog2e, -hi);
@@ -396,11 +452,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_xent_mma(const __grid_constant_
           __syncwarp();
         }
       }
-      fence_before();
-      __syncwarp();
-      if (lane == 0) {
-        if constexpr (kPair) bar_arrive_at(peer_addr(acc_empty(buf), 0)); else bar_arrive(acc_empty(buf));
-      }
+      release(buf);
       ++tile;
       return true;
     });

@@ -399,6 +399,20 @@ def test_xent_pieces_and_chunks(head, dtype, n, d, v):
     check_xent(head, *xent_inputs(gen(n + d + v), n, d, v, dtype))
 
 
+@pytest.mark.parametrize("n,d,v", [(1, 1233, 4), (40, 2048, 30), (300, 1030, 700), (3000, 600, 2600), (130, 4100, 200)])
+def test_xent_wide_f32(head, n, d, v):
+    # long sums in f32: no further off than 32 U of the gradients' norms, wherever they are formed
+    x, w, labels, dl = xent_inputs(gen(n + d), n, d, v, F32)
+    labels = labels.clamp(0, v - 1)
+    check_xent(head, x, w, labels, dl)
+    loss, lse = head.linear_xent_forward(x, w, labels)
+    dx, dw = head.linear_xent_backward(dl, x, w, labels, lse)
+    r = xent64(x, w, labels, dl)
+    assert float((loss.double() - r["loss"]).norm() / r["loss"].norm()) <= 16 * U
+    assert float((dx.double() - r["dx"]).norm() / r["dx"].norm()) <= 64 * U
+    assert float((dw.double() - r["dw"]).norm() / r["dw"].norm()) <= 64 * U
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16])
 def test_xent_one_factor_for_all_rows(head, dtype):
     # a mean's factor, whose rounding to the inputs' type would be the same for every row: 1 / 1000 is 2.2e-3 off in bf16
