@@ -10,9 +10,9 @@
 // Bound by memory: everything is read, and for clipping read again and
 // written. Tensors are cut into chunks of 1,024 vectors of 16 bytes, dealt to
 // the CTAs in turn, whatever the tensors' sizes (a CTA with a run of chunks of
-// its own kept to 3.4 TB/s). The second reading goes backwards: what the first
-// one left in the L2 cache is the end. Clipping has no kernel for the norm
-// between the two: every CTA adds the first kernel's sums itself.
+// its own, or loads that each had a bound to check, kept to 3.4 TB/s; this is
+// 5.3). Clipping has no kernel for the norm between its two passes: every CTA
+// adds the first one's sums itself.
 #include <algorithm>
 
 #include "hb_head.h"
@@ -206,10 +206,9 @@ __global__ void __launch_bounds__(kClipThreads, kCtasPerSm)
   const float q = max_norm / (all + 1e-6f);
   const float by = q > 1.0f ? 1.0f : q;  // NaN stays NaN
   const uint32_t chunks = t.first[t.count];
-  int i = t.count - 1;
-  for (uint32_t back = blockIdx.x; back < chunks; back += gridDim.x) {
-    const uint32_t c = chunks - 1 - back;
-    while (c < t.first[i]) --i;
+  int i = 0;
+  for (uint32_t c = blockIdx.x; c < chunks; c += gridDim.x) {
+    while (c >= t.first[i + 1]) ++i;
     const uint32_t k = c - t.first[i];
     if (t.dtype[i] == HB_F32) scale_chunk((const float*)t.in[i], (float*)t.out[i], t.n[i], k, by);
     else if (t.dtype[i] == HB_F16) scale_chunk((const __half*)t.in[i], (__half*)t.out[i], t.n[i], k, by);

@@ -39,8 +39,12 @@ namespace head {
 namespace {
 
 constexpr int kGroupThreads = 256;
-// The most threads of a CTA, by the registers of 16 elements a thread.
-constexpr int max_threads(bool block) { return block ? 512 : kGroupThreads; }
+// Who holds a row: a group of lanes, a CTA of which there are two an SM (the
+// forward pass alone: 8,191 x 4,097 f32 take it 50 us, 78 with one; the
+// backward pass's column sums then spill, 116 us for 96), or a larger one. The
+// most threads of each, by the registers of 16 elements a thread.
+enum Holder { kByGroup, kBySmall, kByLarge };
+constexpr int max_threads(int holder) { return holder == kByGroup ? kGroupThreads : holder == kBySmall ? 288 : 512; }
 constexpr int kLoopThreads = 512;
 constexpr uint64_t kParts = 640; // rows of partial sums at most
 
@@ -166,10 +170,10 @@ struct Cta {
   __device__ __forceinline__ float2 sum(float2 v) { return Lanes{32}.sum(gather(Lanes{32}.sum(v))); }
 };
 
-// Stages of the ring: as many as fit beside 512 threads' 16 elements of two
-// tensors.
-template <bool kBlock>
-constexpr int kRingStages = kBlock ? 3 : 4;
+// Stages of the ring: as many as fit beside 16 elements a thread of two
+// tensors (one CTA of 512 threads), or of one (two of 288).
+template <int kHolder>
+constexpr int kRingStages = kHolder == kByLarge ? 3 : 4;
 __device__ __forceinline__ void copy_async_4(void* to, const void* from) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from) : "memory");
 }
@@ -256,14 +260,15 @@ struct RowRing {
 
 // kBlock: a CTA a row, else groups of `size` lanes; N vectors a thread. The
 // CTA's rows are base + group for base = blockIdx.x * rows, + the grid's, ...
-template <typename T, typename P, int V, int N, bool kBlock>
-__global__ void __launch_bounds__(max_threads(kBlock))
+template <typename T, typename P, int V, int N, int kHolder>
+__global__ void __launch_bounds__(max_threads(kHolder), kHolder == kByLarge ? 1 : kHolder == kBySmall || (V == 1 && N == 16) ? 2 : 3)
     k_norm_forward(const T* __restrict__ x, uint64_t x_stride, uint64_t n_rows, uint32_t width, int size,
                    const P* __restrict__ w, const P* __restrict__ b, float eps, T* __restrict__ y,
                    float* __restrict__ mean, float* __restrict__ rstd) {
+  constexpr bool kBlock = kHolder != kByGroup;
+  constexpr int kStages = kRingStages<kHolder>;
   __shared__ float2 s[2][32];
   extern __shared__ __align__(16) unsigned char raw[];
-  constexpr int kStages = kRingStages<kBlock>;
   const Part<V, N, kBlock> p(size, width);
   const RowRing<T, V, N, 1, kStages, kBlock> ring(raw, p);
   const uint32_t rows = kBlock ? 1 : kGroupThreads / size, group = kBlock ? 0 : threadIdx.x / size;
@@ -360,13 +365,14 @@ __global__ void __launch_bounds__(max_threads(kBlock))
 
 // As k_norm_forward over the rows; their dw and db sums go to
 // part[CTA][2][width], or where the grid is one CTA to dw and db.
-template <typename T, typename P, int V, int N, bool kBlock>
-__global__ void __launch_bounds__(max_threads(kBlock))
+template <typename T, typename P, int V, int N, int kHolder>
+__global__ void __launch_bounds__(max_threads(kHolder), kHolder == kByGroup ? 2 : 1)
     k_norm_backward(const T* __restrict__ dy, uint64_t dy_stride, const T* __restrict__ x, uint64_t x_stride,
                     uint64_t n_rows, uint32_t width, int size, const P* __restrict__ w,
                     const float* __restrict__ mean, const float* __restrict__ rstd, T* __restrict__ dx,
                     float* __restrict__ part, P* __restrict__ dw, P* __restrict__ db) {
-  constexpr int kStages = kRingStages<kBlock>;
+  constexpr bool kBlock = kHolder != kByGroup;
+  constexpr int kStages = kRingStages<kHolder>;
   __shared__ float2 s[2][32];
   __shared__ float2 s_stats[kStages][kGroupThreads];  // of a group's row; block: a copy a warp
   extern __shared__ __align__(16) unsigned char raw[];
@@ -603,7 +609,7 @@ NormPlan norm_plan(uint32_t width, uint64_t elem, bool vec) {
   if (n > 32 * most) {
     p.items = (int)most;
     p.size = (int)round_up((n + most - 1) / most, 32);
-    p.shape = p.size <= max_threads(true) ? kCta : kLoop;
+    p.shape = p.size <= max_threads(kByLarge) ? kCta : kLoop;
     return p;
   }
   p.shape = kGroup;
@@ -616,20 +622,23 @@ NormPlan norm_plan(uint32_t width, uint64_t elem, bool vec) {
   return p;
 }
 
-// f(vector length, vectors a thread, whether a CTA holds the row) as constants.
-template <typename T, typename F>
+// f(vector length, vectors a thread, who holds the row) as constants.
+template <typename T, bool kBackward, typename F>
 void with_shape(const NormPlan& p, F&& f) {
   using std::integral_constant;
   const auto items = [&](auto v) {
     constexpr int kMost = 16 / decltype(v)::value;
-    if (p.shape == kCta) return f(v, integral_constant<int, kMost>{}, std::true_type{});
-    if (p.items == 1) return f(v, integral_constant<int, 1>{}, std::false_type{});
-    if (p.items == 2) return f(v, integral_constant<int, 2>{}, std::false_type{});
+    const integral_constant<int, kByGroup> group;
+    if constexpr (!kBackward)
+      if (p.shape == kCta && p.size <= max_threads(kBySmall)) return f(v, integral_constant<int, kMost>{}, integral_constant<int, kBySmall>{});
+    if (p.shape == kCta) return f(v, integral_constant<int, kMost>{}, integral_constant<int, kByLarge>{});
+    if (p.items == 1) return f(v, integral_constant<int, 1>{}, group);
+    if (p.items == 2) return f(v, integral_constant<int, 2>{}, group);
     if constexpr (kMost >= 4)
-      if (p.items == 4) return f(v, integral_constant<int, 4>{}, std::false_type{});
+      if (p.items == 4) return f(v, integral_constant<int, 4>{}, group);
     if constexpr (kMost >= 16) {
-      if (p.items == 8) return f(v, integral_constant<int, 8>{}, std::false_type{});
-      return f(v, integral_constant<int, 16>{}, std::false_type{});
+      if (p.items == 8) return f(v, integral_constant<int, 8>{}, group);
+      return f(v, integral_constant<int, 16>{}, group);
     }
   };
   if (p.vec) items(integral_constant<int, 16 / sizeof(T)>{});
@@ -697,15 +706,16 @@ hb_status hb_layer_norm_forward(int32_t device, const void* x, int32_t dtype, ui
                                                           (const P*)bias, eps, (T*)y, mean, rstd);
       return;
     }
-    with_shape<T>(p, [&](auto v, auto n, auto block) {
+    with_shape<T, false>(p, [&](auto v, auto n, auto holder) {
       constexpr int V = decltype(v)::value, N = decltype(n)::value;
-      constexpr bool kBlock = decltype(block)::value;
+      constexpr int kHolder = decltype(holder)::value;
+      constexpr bool kBlock = kHolder != kByGroup;
       const uint64_t rows = kBlock ? 1 : kGroupThreads / p.size;
       const int threads = kBlock ? p.size : kGroupThreads;
-      const uint32_t bytes = RowRing<T, V, N, 1, kRingStages<kBlock>, kBlock>::bytes(threads, kBlock ? 32 : p.size);
-      const uint64_t grid = std::min<uint64_t>((n_rows + rows - 1) / rows, resident(threads, bytes, N * V * 3 + 30) * sms);
-      allow_shared<k_norm_forward<T, P, V, N, kBlock>>(device, bytes);
-      k_norm_forward<T, P, V, N, kBlock><<<(unsigned)grid, threads, bytes, s>>>(
+      const uint32_t bytes = RowRing<T, V, N, 1, kRingStages<kHolder>, kBlock>::bytes(threads, kBlock ? 32 : p.size);
+      const uint64_t grid = std::min<uint64_t>((n_rows + rows - 1) / rows, resident(threads, bytes, kHolder == kBySmall ? 112 : N * V * 3 + 30) * sms);
+      allow_shared<k_norm_forward<T, P, V, N, kHolder>>(device, bytes);
+      k_norm_forward<T, P, V, N, kHolder><<<(unsigned)grid, threads, bytes, s>>>(
           (const T*)x, x_stride, n_rows, width, p.size, (const P*)weight, (const P*)bias, eps, (T*)y, mean, rstd);
     });
   });
@@ -764,17 +774,18 @@ hb_status hb_layer_norm_backward(int32_t device, const void* dy, uint64_t dy_str
         k_norm_slices<T><<<dim3((width + 127) / 128, (unsigned)grid), 128, 0, s>>>((const T*)dy, dy_stride, (const T*)x, x_stride,
                                                                              n_rows, width, mean, rstd, part);
     } else {
-      with_shape<T>(p, [&](auto v, auto n, auto block) {
+      with_shape<T, true>(p, [&](auto v, auto n, auto holder) {
         constexpr int V = decltype(v)::value, N = decltype(n)::value;
-        constexpr bool kBlock = decltype(block)::value;
+        constexpr int kHolder = decltype(holder)::value;
+      constexpr bool kBlock = kHolder != kByGroup;
         const uint64_t rows = kBlock ? 1 : kGroupThreads / p.size;
         const int threads = kBlock ? p.size : kGroupThreads;
-        const uint32_t ring = RowRing<T, V, N, 2, kRingStages<kBlock>, kBlock>::bytes(threads, kBlock ? 32 : p.size);
+        const uint32_t ring = RowRing<T, V, N, 2, kRingStages<kHolder>, kBlock>::bytes(threads, kBlock ? 32 : p.size);
         const uint32_t bytes = kBlock ? ring : std::max<uint32_t>(ring, 8 * (kGroupThreads / 32) * width);
         const uint64_t most = std::min<uint64_t>(kParts, resident(threads, bytes, N * V * 5 + 35) * sms);
         grid = std::min<uint64_t>((n_rows + rows - 1) / rows, most);
-        allow_shared<k_norm_backward<T, P, V, N, kBlock>>(device, bytes);
-        k_norm_backward<T, P, V, N, kBlock><<<(unsigned)grid, threads, bytes, s>>>(
+        allow_shared<k_norm_backward<T, P, V, N, kHolder>>(device, bytes);
+        k_norm_backward<T, P, V, N, kHolder><<<(unsigned)grid, threads, bytes, s>>>(
             (const T*)dy, dy_stride, (const T*)x, x_stride, n_rows, width, p.size, (const P*)weight, mean, rstd, (T*)dx, part,
             (P*)dweight, (P*)dbias);
       });
