@@ -435,8 +435,8 @@ hb_status hb_engine_upload_csr(hb_engine* e, const uint64_t* indptr, const uint3
  * stream). They enqueue their kernels there and return without waiting;
  * they allocate nothing, keep nothing between calls and put the calling
  * thread's current device back. Where a call needs scratch, the matching
- * *_workspace function gives the bytes, and the scratch must stay untouched
- * until the stream has passed the call. Different calls may run at the same
+ * *_workspace function gives the bytes (0: none is wanted), and the scratch
+ * must stay untouched until the stream has passed the call. Different calls may run at the same
  * time if their workspaces and outputs do not overlap. Outputs must not
  * overlap inputs unless said. Results do not change from run to run.
  * HB_INVALID_ARGUMENT (the reason in hb_head_last_error) leaves everything
