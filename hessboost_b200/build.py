@@ -21,7 +21,7 @@ NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-O3", "-lineinfo", "-std=c++17", "-fmad=false",
-    "-Xcompiler", "-fPIC,-O3", "-shared", "-ccbin", "/usr/bin/g++",
+    "-Xcompiler", "-fPIC,-O3", "-shared", "-ccbin", "/usr/bin/g++", "--threads", "0",
 ]
 
 
