@@ -22,6 +22,13 @@ struct MmaOut {
   void* to;
 };
 
+// Pieces (bf16) of G. One, rounded as dx and dw are, would not do for bf16
+// layers either: a row of G sums to 0 over the classes, so what their weights
+// share cancels in dx, but the roundings of G times it do not. Weights of 8
+// with a spread of 0.25 then leave 5% of dx; with two pieces it is 2^-8 of
+// that, and bf16 weights have no finer spread. Both products are done twice
+// for it: 8,192 x 1,024 rows with 50,021 classes take 4.3 ms, 2.6 with one.
+constexpr int kGradPlanesBf16 = 2, kGradPlanesF32 = 3;
 constexpr int kMmaDepth = 2;  // blocks of 64 of k in a stage
 constexpr int kXentChunk = 4; // stages of z's k that f32 operands are summed over in the tensor cores
 
@@ -45,7 +52,7 @@ struct MmaParams {
   CUtensorMap g_out;           // what grad writes (dx and dw read an earlier launch's)
   MmaJob jobs[kMaxJobs];
   int n_jobs;
-  int planes, g_planes;        // of x and w 1: bf16; 3: f32 in three pieces; G's: 1 to 3
+  int planes;                  // of x and w 1: bf16; 3: f32 in three pieces
   int width;
   const void* labels;          // of the call's rows, as the next three
   int label_type;

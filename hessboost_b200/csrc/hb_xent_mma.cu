@@ -55,21 +55,9 @@ struct Shape {
 constexpr float kLog2e = 1.4426950408889634f;
 
 // (piece of A, piece of B) of the products, smallest first; the last one
-// alone for bf16 operands, the last two where G is in two pieces.
+// alone for bf16 operands' logits, the last two where A is bf16's G.
 __constant__ int kPairA[6] = {2, 0, 1, 0, 1, 0};
 __constant__ int kPairB[6] = {0, 2, 1, 1, 0, 0};
-
-// The mantissa, in [1, 2), of the first row's factor: G is formed in units
-// of it and dx and dw multiplied by it again in f32. A factor that is the
-// same for every row (a mean) then does not round each element of a bf16 G
-// the same way, which would not average out: with random factors the
-// gradients are 1.41 of one rounding off, with 1 / n up to 2.4.
-template <bool kSplit>
-__device__ __forceinline__ float unit_of(const MmaParams& p) {
-  const uint32_t bits = __float_as_uint(p.dloss[0]);
-  const uint32_t e = bits >> 23 & 0xffu;
-  return kSplit || e == 0u || e == 0xffu ? 1.0f : __uint_as_float((bits & 0x7fffffu) | 0x3f800000u);
-}
 
 // Stages of a chunk of z's k, and the chunks of a tile.
 constexpr int kChunk = kXentChunk;
@@ -134,7 +122,7 @@ __device__ __forceinline__ void store32(T* dst, const float (&v)[32], int n, boo
 template <bool kPair, bool kSplit>
 __global__ void __launch_bounds__(kThreads, 1) k_xent_mma(const __grid_constant__ MmaParams p) {
   using S = Shape<kPair>;
-  constexpr int kStages = S::kStages;
+  constexpr int kStages = S::kStages, kGradPlanes = kSplit ? kGradPlanesF32 : kGradPlanesBf16;
   extern __shared__ unsigned char raw[];
   const uint32_t base = (smem_addr(raw) + 1023u) & ~1023u;
   const uint32_t staging = base + kStages * S::kStageBytes;
@@ -147,7 +135,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_xent_mma(const __grid_constant_
   const auto acc_empty = [&](int b) { return bars + 8u * (2 * kStages + 2 + b); };
   __shared__ uint32_t s_tmem;
   __shared__ volatile uint32_t s_gave_up;
-  const auto pairs_of = [&](const MmaJob& job) { return kSplit ? 6 : job.kind == kJobDx || job.kind == kJobDw ? p.g_planes : 1; };
+  const auto pairs_of = [&](const MmaJob& job) { return kSplit ? 6 : job.kind == kJobDx || job.kind == kJobDw ? kGradPlanes : 1; };
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = kPair ? blockIdx.x & 1 : 0, worker = blockIdx.x / S::kCtas;
   if (threadIdx.x == 0) {
@@ -349,7 +337,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_xent_mma(const __grid_constant_
         const int64_t label = in ? p.label((int64_t)job.row0 + row) : -1;
         const int64_t rel = label - job.class0 - col0;
         // a row without a label: logits and lse 0 (its operand row is 0), factor 0
-        const float each = !ok ? NAN : label >= 0 ? p.dloss[(size_t)(job.row0 + row) * p.dloss_stride] / unit_of<kSplit>(p) : 0.0f;
+        const float each = !ok ? NAN : label >= 0 ? p.dloss[(size_t)(job.row0 + row) * p.dloss_stride] : 0.0f;
         // exp(z - lse) = 2^(z log2(e) - lse log2(e)). For f32, whose rounding of
         // that difference (about -13 here and there) would be 3e-7 of the
         // result: lse log2(e) = hi + lo with hi a multiple of 2^-9, whole parts
@@ -387,7 +375,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_xent_mma(const __grid_constant_
             for (int i = 0; i < 64; ++i) v[i] = i < left ? v[i] : 0.0f;
           }
 #pragma unroll 1
-          for (int q = 0; q < p.g_planes; ++q) {
+          for (int q = 0; q < kGradPlanes; ++q) {
             if (lane == 0) tma_wait_read<0>();
             __syncwarp();
 #pragma unroll
@@ -397,10 +385,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_xent_mma(const __grid_constant_
               for (int j = 0; j < 4; ++j) {
                 const __nv_bfloat162 b = __floats2bfloat162_rn(v[8 * i + 2 * j], v[8 * i + 2 * j + 1]);
                 h[j] = *reinterpret_cast<const uint32_t*>(&b);
-                if (kSplit || p.g_planes > 1) {
-                  v[8 * i + 2 * j] -= __low2float(b);
-                  v[8 * i + 2 * j + 1] -= __high2float(b);
-                }
+                v[8 * i + 2 * j] -= __low2float(b);
+                v[8 * i + 2 * j + 1] -= __high2float(b);
               }
               asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(stage + lane * 128 + ((i ^ (lane & 7)) << 4)), "r"(h[0]),
                            "r"(h[1]), "r"(h[2]), "r"(h[3])
@@ -418,7 +404,6 @@ __global__ void __launch_bounds__(kThreads, 1) k_xent_mma(const __grid_constant_
         const int rows = job.kind == kJobDx ? job.n_rows : job.n_classes;
         const MmaOut& o = job.out;
         // no step of k fell to an empty split: its accumulator is not written
-        const float unit = !ok ? NAN : unit_of<kSplit>(p);
         const bool none = at.k0 == at.k1;
         for (int c = c0; c < c1; c += 32) {
           const int left = p.width - (col0 + c);
@@ -426,7 +411,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_xent_mma(const __grid_constant_
           float v[32];
           tmem_load32(acc + c, v);
 #pragma unroll
-          for (int i = 0; i < 32; ++i) v[i] = none ? 0.0f : v[i] * unit;
+          for (int i = 0; i < 32; ++i) v[i] = !ok ? NAN : none ? 0.0f : v[i];
           if (row < rows) {
             const int n = left < 32 ? left : 32;
             if (o.type == kOutAcc) {
@@ -498,13 +483,15 @@ namespace {
 
 // Shares the jobs' tiles out among the workers in the jobs' order: each
 // job's tiles go where the least work is so far (a tile's work: its blocks
-// of k and about three more), as far as whole tiles allow.
+// of k, times the products of pieces, and about three more), as far as whole
+// tiles allow.
 void share_out(MmaParams& p, int workers) {
   long long load[kMaxWorkers] = {};
   for (int j = 0; j < p.n_jobs; ++j) {
     const MmaJob& job = p.jobs[j];
     const long long tiles = (long long)job.m_tiles * job.n_tiles * job.splits;
-    const long long cost = (p.planes > 1 ? 6ll : 1ll) * kMmaDepth * job.k_blocks / job.splits + 3;
+    const long long pairs = p.planes > 1 ? 6 : job.kind == kJobDx || job.kind == kJobDw ? kGradPlanesBf16 : 1;
+    const long long cost = pairs * kMmaDepth * job.k_blocks / job.splits + 3;
     const auto below = [&](long long level) {
       long long n = 0;
       for (int u = 0; u < workers; ++u) n += level > load[u] ? (level - load[u]) / cost : 0;

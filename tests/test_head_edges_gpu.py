@@ -1,0 +1,83 @@
+"""The embedding-head operators (hessboost_b200/head.py) where their sums cancel, run long or leave a type's range,
+against plain 64-bit formulas. u is the unit roundoff of a type (f32 2^-24, bf16 2^-8) and U = 2^-24 that of f32 sums."""
+
+import math
+
+import pytest
+
+torch = pytest.importorskip("torch")
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0**-24
+F32, BF16 = torch.float32, torch.bfloat16
+UNIT = {F32: 2.0**-24, BF16: 2.0**-8}
+
+
+@pytest.fixture(scope="module")
+def head():
+    from hessboost_b200 import head as h
+
+    return h
+
+
+def gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def rand(g, *shape, dtype=F32, by=1.0):
+    return (torch.randn(*shape, generator=g, device="cuda") * by).to(dtype)
+
+
+def xent64(x, w, labels, dloss):
+    """loss, |G|, dx and dw in 64 bits; every label is a class."""
+    x, w = x.double(), w.double()
+    z = x @ w.T
+    at = labels.long()[:, None]
+    zl = z.gather(1, at)[:, 0]
+    # log sum exp(z - z_label): no cancellation where the label's logit is all there is
+    rest = (z - zl[:, None]).scatter(1, at, -math.inf)
+    loss = torch.logaddexp(torch.zeros_like(zl), torch.logsumexp(rest, 1))
+    g = torch.softmax(z, 1)
+    g.scatter_add_(1, at, -torch.ones_like(at, dtype=torch.float64))
+    g *= dloss.double()[:, None]
+    return dict(z=z, loss=loss, g=g, dx=g @ w, dw=g.T @ x)
+
+
+def off(got, want):
+    return float((got.double() - want).norm() / want.norm())
+
+
+@pytest.mark.parametrize("n,d,v", [(600, 64, 3000), (257, 72, 500), (5000, 128, 700)])
+def test_xent_gradient_of_weights_with_a_common_offset(head, n, d, v):
+    # a row of G sums to 0, so what all the classes' weights share cancels in dx = G w
+    g = gen(n + v)
+    x, w = rand(g, n, d, by=0.125), (8 + rand(g, v, d, by=0.25)).to(BF16)
+    x = (x - x.mean(1, keepdim=True)).to(BF16)
+    labels = torch.randint(v, (n,), generator=g, device="cuda")
+    dl = (0.5 + torch.rand(n, generator=g, device="cuda")) / n
+    _, lse = head.linear_xent_forward(x, w, labels)
+    dx, dw = head.linear_xent_backward(dl, x, w, labels, lse)
+    r = xent64(x, w, labels, dl)
+    u = UNIT[BF16]
+    # the output's rounding (0.6 u of the norm: elements at their worst are u / sqrt 3); two roundings of G's elements (u
+    # each of what the first leaves), which do not cancel; and p's error, that of logits added up 16 products at a time
+    # (2 U of at most the sum of magnitudes each) and of lse
+    z_off = (d / 16 + 2) * 2 * U * float((x.double().abs() @ w.double().abs().T).max())
+    assert off(dx, r["dx"]) <= 0.6 * u + (u * u + z_off) * float((r["g"].abs() @ w.double().abs()).norm() / r["dx"].norm())
+    assert off(dw, r["dw"]) <= 0.6 * u + (u * u + z_off) * float((r["g"].T.abs() @ x.double().abs()).norm() / r["dw"].norm())
+
+
+@pytest.mark.parametrize("first", [0.0, 1e-3, 1.0])
+def test_xent_one_factor_for_all_rows_but_the_first(head, first):
+    # a mean over the rows that count: 1 / 1000 rounded to bf16 once would be 2.2e-3 off in every element of G alike
+    g = gen(25)
+    x, w = rand(g, 1000, 64, dtype=BF16), rand(g, 500, 64, dtype=BF16, by=0.125)
+    labels = torch.randint(500, (1000,), generator=g, device="cuda")
+    dl = torch.full((1000,), 1e-3, device="cuda")
+    dl[0] = first
+    _, lse = head.linear_xent_forward(x, w, labels)
+    dx, dw = head.linear_xent_backward(dl, x, w, labels, lse)
+    r = xent64(x, w, labels, dl)
+    assert off(dx, r["dx"]) <= 0.75 * UNIT[BF16] + 64 * U
+    assert off(dw, r["dw"]) <= 0.75 * UNIT[BF16] + 64 * U
