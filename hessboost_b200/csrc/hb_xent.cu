@@ -6,8 +6,8 @@
 // A label outside [0, n_classes) is a row without a label: its loss is 0
 // and it takes no part in the gradients. The forward pass keeps only lse;
 // the backward pass computes the logits again, a piece of the classes (and a
-// chunk of the rows) at a time, so that what is held of G stays below
-// kGradElements. The products are hb_xent_mma.cu's.
+// chunk of the rows) at a time, so that what is held of G stays below a fixed
+// number of elements. The products are hb_xent_mma.cu's.
 #include <algorithm>
 #include <cmath>
 
@@ -17,11 +17,12 @@ namespace hb {
 namespace head {
 namespace {
 
-// Elements of G's pieces held at a time (160 MiB): with half as many, twice
-// the launches, 8,192 x 1,024 bf16 rows with 50,021 classes take 4.7 ms for
-// 4.3 and 4,099 x 257 f32 rows with 12,289 classes 813 us for 791; 2,048 x
-// 2,048 bf16 rows with 32,000 classes take 1.23 ms for 1.30.
-constexpr int64_t kGradElements = 80ll << 20;
+// Elements of G's pieces held at a time (160 MiB in bf16): with half as many,
+// twice the launches, 8,192 x 1,024 bf16 rows with 50,021 classes take 4.7 ms
+// for 4.3, 2,048 x 2,048 with 32,000 classes 1.23 for 1.30. In f32 as many
+// would make 4,099 x 257 rows with 12,289 classes 791 us for 813, but the
+// chunks of rows, and with them the parts that dw is summed in, twice as many.
+constexpr int64_t kGradElementsBf16 = 80ll << 20, kGradElementsF32 = 40ll << 20;
 constexpr uint64_t kPartBytes = 64ull << 20;   // of the stats' parts held at a time
 constexpr int kFinishThreads = 256;
 
@@ -186,14 +187,17 @@ int last_cols(uint64_t cols, int n, bool pair) {
     if (share * ctas >= left && share * ctas <= n) return share * ctas;
   return n;
 }
-// Parts of k: enough tiles for the workers, at least 4 steps of 64 each. In
-// f32 a part is at most 1,024 long: the tensor cores' own sums round towards
-// zero, and over 4,099 rows that was 2e-6 of dw, twice what f32 sums that
-// round to nearest are off.
+// Parts of k: enough tiles for the workers, at least 4 steps of 64 each, and
+// none longer than its type's sums may be, since the tensor cores' own sums
+// round towards zero. In f32 that is 1,024: dw of 131,072 to 600,000 rows is
+// then 15 to 23 U off (U = 2^-24; plain f32 sums 4 to 11), whatever its terms'
+// signs; with parts of 2,600 it was 50 to 99 U, of 8,100 140 to 500 U. In bf16
+// it is 32,768, some 2^-12 of the result.
 int k_splits(uint64_t tiles, int k_blocks, int workers, int planes) {
   const int want = tiles >= (uint64_t)workers ? 1 : (int)((workers + tiles - 1) / tiles);
   const int by_tiles = std::max(1, std::min(want, k_blocks * kMmaDepth / 4));
-  return planes == 1 ? by_tiles : std::max(by_tiles, std::min(32, (k_blocks * kMmaDepth * 64 + 1023) / 1024));
+  const int longest = (planes == 1 ? 32768 : 1024) / (64 * kMmaDepth);  // in k_blocks
+  return std::max(by_tiles, (k_blocks + longest - 1) / longest);
 }
 
 struct Forward {
@@ -233,7 +237,7 @@ Backward backward_plan(const Sizes& z, int32_t dtype, const void* x, uint64_t x_
   Backward b;
   b.x = operand_of(z, dtype, x, x_stride, z.n_rows, true);
   b.w = operand_of(z, dtype, w, w_stride, z.n_classes, false);
-  const uint64_t most = (uint64_t)kGradElements / z.g_planes;
+  const uint64_t most = (uint64_t)(z.planes == 1 ? kGradElementsBf16 : kGradElementsF32) / z.g_planes;
   const uint64_t least = 2048;  // classes of a piece, where there are as many
   b.chunk = std::min(z.n_rows, std::max<uint64_t>(most / std::min(z.n_classes, least) / 256 * 256, 256));
   b.chunks = (z.n_rows + b.chunk - 1) / b.chunk;

@@ -81,3 +81,19 @@ def test_xent_one_factor_for_all_rows_but_the_first(head, first):
     r = xent64(x, w, labels, dl)
     assert off(dx, r["dx"]) <= 0.75 * UNIT[BF16] + 64 * U
     assert off(dw, r["dw"]) <= 0.75 * UNIT[BF16] + 64 * U
+
+
+@pytest.mark.parametrize("one_sign", [False, True])
+@pytest.mark.parametrize("n,d,v", [(4096, 600, 64), (300000, 1024, 40), (600000, 600, 20)])
+def test_xent_long_sums_in_f32(head, n, d, v, one_sign):
+    # dw sums over the rows, which the tensor cores would round towards zero at every step. A part of 1,024 has 64 steps
+    # of 16, each off by 2 U of what is summed so far at most, 64 U of a sum of terms of one sign; the logits, of about 1
+    # and in parts of 512, have 32, and so has p its relative error of 64 U at most
+    g = gen(n)
+    x = torch.rand(n, d, generator=g, device="cuda") + 0.5 if one_sign else rand(g, n, d)
+    w = rand(g, v, d, by=d**-0.5)
+    labels = torch.zeros(n, dtype=torch.int64, device="cuda") if one_sign else torch.randint(v, (n,), generator=g, device="cuda")
+    dl = torch.full((n,), 1.0 / n, device="cuda")
+    _, lse = head.linear_xent_forward(x, w, labels)
+    dw = head.linear_xent_backward(dl, x, w, labels, lse)[1]
+    assert off(dw, xent64(x, w, labels, dl)["dw"]) <= 128 * U
