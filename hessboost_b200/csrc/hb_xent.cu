@@ -176,7 +176,7 @@ int tile_cols(uint64_t cols, uint64_t m_tiles, int workers, int unit, uint64_t m
 }
 // The most columns of a tile of logits: where k is summed in chunks, as many
 // as an epilogue warp can hold the sums of.
-uint64_t z_cols(const Sizes& z) { return z.planes > 1 && stages_of(z.width) > kXentChunk ? 128 : 256; }
+uint64_t z_cols(const Sizes& z) { return z_chunked(z.planes, z.width) ? 128 : 256; }
 
 // Columns of the last of the tiles of n columns: 16 a CTA, 32, 64, or all,
 // where that is enough (each CTA's share then lies in whole blocks of 64, or

@@ -30,7 +30,11 @@ struct MmaOut {
 // for it: 8,192 x 1,024 rows with 50,021 classes take 4.3 ms, 2.6 with one.
 constexpr int kGradPlanesBf16 = 2, kGradPlanesF32 = 3;
 constexpr int kMmaDepth = 2;  // blocks of 64 of k in a stage
-constexpr int kXentChunk = 4; // stages of z's k that f32 operands are summed over in the tensor cores
+// Stages of z's k that are summed in the tensor cores, and whether there are more.
+constexpr int kXentChunkF32 = 4, kXentChunkBf16 = 16;
+constexpr bool z_chunked(int planes, uint32_t width) {
+  return (width + 64 * kMmaDepth - 1) / (64 * kMmaDepth) > (planes > 1 ? kXentChunkF32 : kXentChunkBf16);
+}
 
 // m_tiles x n_tiles tiles of (128 x CTAs) x n_size (the last ones n_last), k (k_total of it) in
 // k_blocks stages shared among `splits` tiles each; m_fast: consecutive tiles go down the rows.

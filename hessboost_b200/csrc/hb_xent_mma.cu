@@ -23,10 +23,17 @@
 // f32 operands are three bf16 pieces (v = p0 + p1 + p2, each the rounding of
 // what the ones before leave), and a product is the six products of pieces
 // whose orders add up to at most 2: what is left out is below 2^-24 of the
-// operands' product. The smallest are summed first. The tensor cores round
-// their sums towards zero, so a long k is summed in chunks of kChunk stages in
-// f32 arithmetic: z over 1,233 columns in one go left 8e-6 of the gradients
-// (for dx and dw, whose k is cut up anyway, see k_splits).
+// operands' product. The smallest are summed first.
+//
+// The tensor cores round their sums towards zero, so the logits' k, where it
+// is long, is summed in chunks that are added up in f32 arithmetic: f32 in
+// chunks of 512 (z over 1,233 columns in one go left 8e-6 of the gradients),
+// bf16, whose loss is f32 too, in chunks of 2,048: over 16,384 columns in one
+// go the loss was 48 U off (U = 2^-24), now it is 5.3, as over 2,048. An
+// epilogue warp then holds 64 columns' sums, so the tiles are at most 128 wide
+// and fetch more: 2,048 x 4,096 bf16 rows with 32,000 classes take 805 us
+// forward, 515 in one go. (For dx and dw, whose k is cut up anyway, see
+// k_splits.)
 #include <algorithm>
 #include <cmath>
 #include <string>
@@ -59,11 +66,11 @@ constexpr float kLog2e = 1.4426950408889634f;
 __constant__ int kPairA[6] = {2, 0, 1, 0, 1, 0};
 __constant__ int kPairB[6] = {0, 2, 1, 1, 0, 0};
 
-// Stages of a chunk of z's k, and the chunks of a tile.
-constexpr int kChunk = kXentChunk;
-template <bool kSplit>
+// The chunks that a tile's k is summed in.
+template <bool kSplit, bool kChunked>
 __device__ __forceinline__ int chunks_of(const MmaJob& job, int k0, int k1) {
-  return kSplit && (job.kind == kJobStats || job.kind == kJobGrad) ? max(1, (k1 - k0 + kChunk - 1) / kChunk) : 1;
+  constexpr int kChunk = kSplit ? kXentChunkF32 : kXentChunkBf16;
+  return kChunked && (job.kind == kJobStats || job.kind == kJobGrad) ? max(1, (k1 - k0 + kChunk - 1) / kChunk) : 1;
 }
 
 template <int kStages>
@@ -118,10 +125,12 @@ __device__ __forceinline__ void store32(T* dst, const float (&v)[32], int n, boo
   }
 }
 
-// kSplit: f32 operands in three pieces.
-template <bool kPair, bool kSplit>
+// kSplit: f32 operands in three pieces. kChunked: z's k may be longer than a
+// chunk, tiles of z are at most 128 columns wide.
+template <bool kPair, bool kSplit, bool kChunked>
 __global__ void __launch_bounds__(kThreads, 1) k_xent_mma(const __grid_constant__ MmaParams p) {
   using S = Shape<kPair>;
+  constexpr int kChunk = kSplit ? kXentChunkF32 : kXentChunkBf16;
   constexpr int kStages = S::kStages, kGradPlanes = kSplit ? kGradPlanesF32 : kGradPlanesBf16;
   extern __shared__ unsigned char raw[];
   const uint32_t base = (smem_addr(raw) + 1023u) & ~1023u;
@@ -167,7 +176,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_xent_mma(const __grid_constant_
       const int a_row = (at.m * S::kCtas + rank) * 128 + (ma == &p.x_k ? job.row0 : 0);
       const int b_row = at.n * job.n_size + rank * share + (mb == &p.w_k ? job.class0 : 0);
       const int bk0 = mb == &p.w_mn ? job.class0 : mb == &p.x_mn ? job.row0 : 0;
-      const int chunks = chunks_of<kSplit>(job, at.k0, at.k1), pairs = pairs_of(job);
+      const int chunks = chunks_of<kSplit, kChunked>(job, at.k0, at.k1), pairs = pairs_of(job);
       for (int c = 0; c < chunks * pairs; ++c) {
         const int q = 6 - pairs + c % pairs, pa = kPairA[q], pb = kPairB[q];
         const int k0 = chunks > 1 ? at.k0 + c / pairs * kChunk : at.k0, k1 = chunks > 1 ? min(at.k1, k0 + kChunk) : at.k1;
@@ -207,7 +216,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_xent_mma(const __grid_constant_
       // rows on; mn-major: 16 of k are 16 rows of 128 bytes on
       const uint32_t share = job.n_size / S::kCtas;  // k-major tiles are all alike
       const uint32_t block_a = a_mn ? 64 * kRow >> 4 : 128 * kRow >> 4, block_b = b_mn ? 64 * kRow >> 4 : share * kRow >> 4;
-      const int chunks = chunks_of<kSplit>(job, at.k0, at.k1);
+      const int chunks = chunks_of<kSplit, kChunked>(job, at.k0, at.k1);
       for (int c = 0; c < chunks; ++c, ++tile) {
         const int buf = tile & 1;
         if (!bar_wait<kPair>(acc_empty(buf), ((tile >> 1) & 1) ^ 1, &s_gave_up)) return false;
@@ -244,7 +253,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_xent_mma(const __grid_constant_
     int tile = 0;
     each_tile(p, worker, [&](const MmaJob& job, const TileAt& at) {
       const int cut = min(at.cols, (at.cols / 2 + 63) & ~63), c0 = half ? cut : 0, c1 = half ? at.cols : cut;
-      const int chunks = chunks_of<kSplit>(job, at.k0, at.k1);
+      const int chunks = chunks_of<kSplit, kChunked>(job, at.k0, at.k1);
       const auto release = [&](int buf) {
         fence_before();
         __syncwarp();
@@ -253,9 +262,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_xent_mma(const __grid_constant_
         }
       };
       // the chunks but the last, of the warp's 64 columns (tiles are 128 wide at most)
-      float sum[kSplit ? 64 : 1] = {};
+      float sum[kChunked ? 64 : 1] = {};
       bool ok = true;
-      if constexpr (kSplit) {
+      if constexpr (kChunked) {
         for (int c = 0; c + 1 < chunks; ++c, ++tile) {
           const int buf = tile & 1;
           ok = bar_wait(acc_full(buf), (tile >> 1) & 1, &s_gave_up) && ok;
@@ -280,7 +289,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_xent_mma(const __grid_constant_
       const uint32_t acc = tmem + buf * 256 + ((uint32_t)(quarter * 32) << 16);
       // adds the chunks before to the accumulators of columns c and on
       const auto add_chunks = [&](int c, float* v) {
-        if constexpr (kSplit) {
+        if constexpr (kChunked) {
           if (chunks > 1) {
 #pragma unroll
             for (int i = 0; i < 32; ++i) v[i] += c == c0 ? sum[i] : sum[32 + i];
@@ -517,14 +526,14 @@ void share_out(MmaParams& p, int workers) {
   }
 }
 
-template <bool kPair, bool kSplit>
+template <bool kPair, bool kSplit, bool kChunked>
 hb_status launch(const MmaParams& p, int workers, cudaStream_t s) {
   using S = Shape<kPair>;
   static thread_local int ready = -1;
   int device = 0;
   cudaGetDevice(&device);
   if (ready != device) {
-    if (cudaFuncSetAttribute(k_xent_mma<kPair, kSplit>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmemBytes) != cudaSuccess)
+    if (cudaFuncSetAttribute(k_xent_mma<kPair, kSplit, kChunked>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmemBytes) != cudaSuccess)
       return fail(HB_DEVICE_FAILED, "shared memory of the product kernel");
     ready = device;
   }
@@ -538,7 +547,7 @@ hb_status launch(const MmaParams& p, int workers, cudaStream_t s) {
   a[0].val.clusterDim = {S::kCtas, 1, 1};
   c.attrs = a;
   c.numAttrs = kPair ? 1 : 0;
-  const cudaError_t e = cudaLaunchKernelEx(&c, k_xent_mma<kPair, kSplit>, p);
+  const cudaError_t e = cudaLaunchKernelEx(&c, k_xent_mma<kPair, kSplit, kChunked>, p);
   if (e == cudaSuccess) return HB_OK;
   cudaGetLastError();
   return fail(HB_DEVICE_FAILED, std::string("product kernel: ") + cudaGetErrorString(e));
@@ -553,8 +562,9 @@ hb_status mma_launch(MmaParams& p, bool pair, int sms, cudaStream_t s) {
   const int most = std::min(pair ? sms / 2 : sms, kMaxWorkers);
   const int workers = (int)std::min<long long>(tiles, std::max(most, 1));
   share_out(p, workers);
-  if (p.planes > 1) return pair ? launch<true, true>(p, workers, s) : launch<false, true>(p, workers, s);
-  return pair ? launch<true, false>(p, workers, s) : launch<false, false>(p, workers, s);
+  if (p.planes > 1) return pair ? launch<true, true, true>(p, workers, s) : launch<false, true, true>(p, workers, s);
+  if (z_chunked(p.planes, p.width)) return pair ? launch<true, false, true>(p, workers, s) : launch<false, false, true>(p, workers, s);
+  return pair ? launch<true, false, false>(p, workers, s) : launch<false, false, false>(p, workers, s);
 }
 
 }  // namespace head

@@ -97,3 +97,19 @@ def test_xent_long_sums_in_f32(head, n, d, v, one_sign):
     _, lse = head.linear_xent_forward(x, w, labels)
     dw = head.linear_xent_backward(dl, x, w, labels, lse)[1]
     assert off(dw, xent64(x, w, labels, dl)["dw"]) <= 128 * U
+
+
+@pytest.mark.parametrize("n,d,v", [(130, 2056, 700), (512, 4096, 3000), (300, 16384, 1000), (3000, 4100, 2600)])
+def test_xent_logits_of_wide_bf16_rows(head, n, d, v):
+    # the loss is f32: logits of about 1 in parts of 2,048, 128 steps of 16 each off by 2 U of what is summed so far (half
+    # of the part's sum on average): 128 U of a logit at most, 16 U of a loss of log v
+    g = gen(d)
+    x, w = rand(g, n, d, dtype=BF16), rand(g, v, d, dtype=BF16, by=d**-0.5)
+    labels = torch.randint(v, (n,), generator=g, device="cuda")
+    dl = (0.5 + torch.rand(n, generator=g, device="cuda")) / n
+    loss, lse = head.linear_xent_forward(x, w, labels)
+    r = xent64(x, w, labels, dl)
+    assert off(loss, r["loss"]) <= 16 * U
+    assert off(lse, torch.logsumexp(r["z"], 1)) <= 16 * U
+    dx, dw = head.linear_xent_backward(dl, x, w, labels, lse)
+    assert off(dx, r["dx"]) <= 0.75 * UNIT[BF16] + 128 * U and off(dw, r["dw"]) <= 0.75 * UNIT[BF16] + 128 * U
