@@ -181,10 +181,13 @@ __global__ void __launch_bounds__(kForwardThreads, N * V <= 8 ? 4 : N * V <= 16 
   // the warp's lanes stay together: as many rounds as its longest row has
   int rounds = begin < end ? (int)((end - begin + kBatch * split - 1) / (kBatch * split)) : 0;
   rounds = __reduce_max_sync(0xffffffffu, rounds);
-  for (uint32_t c = begin; rounds > 0; --rounds, c += kBatch * split) {
+  // a group whose own row is through stays where it is: going on, `c` could
+  // pass 2^32 and come back to cells before `end`
+  for (uint32_t c = begin; rounds > 0; --rounds) {
     constexpr int U = kFlight / N;  // cells in flight
     ids = next;
-    if (rounds > 1) fetch(c + kBatch * split);
+    if (c < end) c += kBatch * split;  // less than 256 past the end, and 2^32 is 4,098 past it
+    if (rounds > 1) fetch(c);
     const bool whole = __all_sync(0xffffffffu, ids.all([&](uint32_t t) { return t < n_tokens; }));
 #pragma unroll
     for (int b = 0; b < kBatch; b += U) {

@@ -113,3 +113,20 @@ def test_xent_logits_of_wide_bf16_rows(head, n, d, v):
     assert off(lse, torch.logsumexp(r["z"], 1)) <= 16 * U
     dx, dw = head.linear_xent_backward(dl, x, w, labels, lse)
     assert off(dx, r["dx"]) <= 0.75 * UNIT[BF16] + 128 * U and off(dw, r["dw"]) <= 0.75 * UNIT[BF16] + 128 * U
+
+
+def test_embed_cells_near_32_bits(head):
+    # rows of one warp go on together: a short row beside a long one, both within the long one's length of 2^32 cells
+    cells = 2**32 - 5000
+    if torch.cuda.mem_get_info()[0] < 6 * cells:
+        pytest.skip("needs 26 GB")
+    tok = torch.full((cells,), -1, dtype=torch.int32, device="cuda")
+    tok[:200000] = 1  # of no row
+    at = [cells - 110000, cells - 10000, cells - 9990, cells - 9990, cells - 9000, cells]
+    tok[at[0]:] = 0
+    tok[at[1]:at[2]] = 2
+    # so many rows that a warp takes several; the others are empty, before and after
+    ptr = torch.tensor([at[0]] * 8 + at + [cells] * 40000, device="cuda")
+    out = head.embed_forward(tok, torch.eye(3, device="cuda"), row_ptr=ptr)
+    assert out[8:13].tolist() == [[100000, 0, 0], [0, 0, 10], [0, 0, 0], [990, 0, 0], [9000, 0, 0]]
+    assert (out[:8] == 0).all() and (out[13:] == 0).all()
