@@ -103,9 +103,11 @@ __global__ void __launch_bounds__(32 * kJoinWarps)
   __syncthreads();
   if (warp || r >= n_rows) return;
   for (int i = 1; i < kJoinWarps; ++i) a = joined(a, sh[i][lane]);
-  const float l = a.x + logf(a.y);
-  lse[r] = l;
-  loss[r] = label_of(labels, r, n_classes) >= 0 ? l - at_label[r] : 0.0f;
+  // a.y is at least 1, the maximum's own term, and the label's logit at most
+  // the maximum: the loss is not below 0
+  const float rest = logf(a.y);
+  lse[r] = a.x + rest;
+  loss[r] = label_of(labels, r, n_classes) >= 0 ? (a.x - at_label[r]) + rest : 0.0f;
 }
 
 // out[r][d] = the sum of the splits' accumulators, in their order; a thread

@@ -138,9 +138,9 @@ __global__ void __launch_bounds__(kFewThreads) k_few_forward(const FewParams p) 
     for (int s = F::kLanes / 2; s; s >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
     const float at = __shfl_sync(0xffffffffu, z, k * F::kLanes + max(label, 0));
     if (v == 0 && in) {
-      const float lse = from + logf(sum);
-      p.lse[r] = lse;
-      p.loss[r] = label >= 0 ? lse - at : 0.0f;
+      const float rest = logf(sum);
+      p.lse[r] = from + rest;
+      p.loss[r] = label >= 0 ? (from - at) + rest : 0.0f;  // lse's rounding, of the logits' size, plays no part
     }
   }
 }

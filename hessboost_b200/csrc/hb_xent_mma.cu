@@ -61,6 +61,20 @@ struct Shape {
 };
 constexpr float kLog2e = 1.4426950408889634f;
 
+// exp(x), and a = exp(a - ref), b = exp(b - ref). The softmax statistics take
+// the difference first, in which logits near the maximum are exact, and the
+// maximum's own term is 1 whatever its size: a term of 2^(x log2(e) - the
+// rounded ref log2(e)) made the loss of certain rows negative and overflowed
+// with logits near the type's limits.
+__device__ __forceinline__ float exp_fast(float x) { return exp2_fast(x * kLog2e); }
+__device__ __forceinline__ void exp_fast2(float& a, float& b, float ref) {
+  float2 v = make_float2(a, b), r = make_float2(-ref, -ref), l = make_float2(kLog2e, kLog2e);
+  unsigned long long& u = reinterpret_cast<unsigned long long&>(v);
+  asm("add.rn.f32x2 %0, %0, %1;" : "+l"(u) : "l"(reinterpret_cast<unsigned long long&>(r)));
+  asm("mul.rn.f32x2 %0, %0, %1;" : "+l"(u) : "l"(reinterpret_cast<unsigned long long&>(l)));
+  a = exp2_fast(v.x), b = exp2_fast(v.y);
+}
+
 // (piece of A, piece of B) of the products, smallest first; the last one
 // alone for bf16 operands' logits, the last two where A is bf16's G.
 __constant__ int kPairA[6] = {2, 0, 1, 0, 1, 0};
@@ -323,10 +337,13 @@ __global__ void __launch_bounds__(kThreads, 1) k_xent_mma(const __grid_constant_
 #pragma unroll
           for (int i = 3; i < 32; ++i) t[i & 3] = fmaxf(t[i & 3], v[i]);
           const float top = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
-          const float ref = top == -INFINITY ? 0.0f : top * kLog2e;
-          float add[4] = {s * exp2_fast(fmaf(m, kLog2e, -ref)), 0.0f, 0.0f, 0.0f};
+          const float ref = top == -INFINITY ? 0.0f : top;
+          float add[4] = {s * exp_fast(m - ref), 0.0f, 0.0f, 0.0f};
 #pragma unroll
-          for (int i = 0; i < 32; ++i) add[i & 3] += exp2_fast(fmaf(v[i], kLog2e, -ref));
+          for (int i = 0; i < 32; i += 2) {
+            exp_fast2(v[i], v[i + 1], ref);
+            add[i & 3] += v[i], add[(i & 3) + 1] += v[i + 1];
+          }
           s = (add[0] + add[1]) + (add[2] + add[3]);
           m = top;
         }
@@ -337,8 +354,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_xent_mma(const __grid_constant_
         if (!half && in) {
           float2 o;
           asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(o.x), "=f"(o.y) : "r"(meet) : "memory");
-          const float top = fmaxf(m, o.x), ref = top == -INFINITY ? 0.0f : top * kLog2e;
-          s = s * exp2_fast(fmaf(m, kLog2e, -ref)) + o.y * exp2_fast(fmaf(o.x, kLog2e, -ref));
+          const float top = fmaxf(m, o.x), ref = top == -INFINITY ? 0.0f : top;
+          s = s * exp_fast(m - ref) + o.y * exp_fast(o.x - ref);
           p.part[(size_t)at.n * p.part_stride + row] = ok ? make_float2(top, s) : make_float2(NAN, NAN);
         }
       } else if (job.kind == kJobGrad) {

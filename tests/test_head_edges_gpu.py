@@ -130,3 +130,48 @@ def test_embed_cells_near_32_bits(head):
     out = head.embed_forward(tok, torch.eye(3, device="cuda"), row_ptr=ptr)
     assert out[8:13].tolist() == [[100000, 0, 0], [0, 0, 10], [0, 0, 0], [990, 0, 0], [9000, 0, 0]]
     assert (out[:8] == 0).all() and (out[13:] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("d,v", [(64, 12), (64, 3000), (200, 500)])
+@pytest.mark.parametrize("near", [0.0, 0.9])
+def test_xent_loss_of_certain_rows(head, dtype, d, v, near):
+    # logits of 20 to 200, the label's far above the rest, or a little above one other: the loss is what the rest add to
+    # 1, and never below 0
+    g = gen(v)
+    w = rand(g, v, d, dtype=dtype)
+    labels = torch.randint(v, (4000,), generator=g, device="cuda")
+    by = (20 + 180 * torch.rand(4000, 1, generator=g, device="cuda")) / d
+    x = ((w[labels].float() + near * w[labels - 1].float()) * by).to(dtype)
+    loss, lse = head.linear_xent_forward(x, w, labels)
+    r = xent64(x, w, labels, torch.ones(4000, device="cuda"))
+    assert float(loss.min()) >= 0, (int((loss < 0).sum()), float(loss.min()))
+    # each of the rest's terms is off by the logits' own error (d products); their sum and log by (v / 32 + 32) U, and
+    # their terms' exponents by one rounding
+    dz = (d + 4) * U * (x.double().abs() @ w.double().abs().T).max(1).values
+    assert ((loss.double() - r["loss"]).abs() <= (r["loss"] + 32 * U) * torch.expm1(2 * dz) + (v / 32 + 32) * U + 2 * U * r["loss"]).all()
+
+
+def masked_by_the_lowest_value(head, dtype, v, kept):
+    # a column of ones makes the weights' last column a bias; the type's lowest value there masks a class, here whole
+    # tiles of them: the others' loss and gradients are those of a layer without it
+    g = gen(v)
+    n, d = 300, 64
+    x, w = rand(g, n, d, dtype=dtype), rand(g, v, d, dtype=dtype, by=0.125)
+    x[:, -1] = 1
+    keep = torch.arange(v, device="cuda") < kept
+    w[~keep, -1] = torch.finfo(dtype).min
+    labels = torch.randint(kept, (n,), generator=g, device="cuda")
+    dl = (0.5 + torch.rand(n, generator=g, device="cuda")) / n
+    loss, lse = head.linear_xent_forward(x, w, labels)
+    dx, dw = head.linear_xent_backward(dl, x, w, labels, lse)
+    r = xent64(x, w[keep], labels, dl)
+    tol = 0.75 * UNIT[dtype] + 64 * U
+    assert off(loss, r["loss"]) <= 64 * U
+    assert off(dx, r["dx"]) <= tol and off(dw[keep], r["dw"]) <= tol
+    assert (dw[~keep] == 0).all()
+
+
+@pytest.mark.parametrize("v,kept", [(20, 7), (2049, 200), (5000, 2700)])
+def test_xent_classes_masked_by_the_lowest_value_bf16(head, v, kept):
+    masked_by_the_lowest_value(head, BF16, v, kept)
