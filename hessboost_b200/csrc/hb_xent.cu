@@ -67,7 +67,9 @@ __global__ void k_xent_pack(const T* __restrict__ x, uint64_t x_stride, uint64_t
       Pack<__nv_bfloat16, 8> b;
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        b.v[j] = __float2bfloat16_rn(v[j]);
+        // f32 past bf16's largest value: the first piece is that, not infinity
+        const float most = 0x1.fep127f, size = fabsf(v[j]);
+        b.v[j] = __float2bfloat16_rn(kPlanes > 1 && size > most && size < INFINITY ? copysignf(most, v[j]) : v[j]);
         if (q + 1 < kPlanes) v[j] -= __bfloat162float(b.v[j]);
       }
       *reinterpret_cast<Pack<__nv_bfloat16, 8>*>(out + (q * n_rows + r) * padded + d) = b;

@@ -175,3 +175,8 @@ def masked_by_the_lowest_value(head, dtype, v, kept):
 @pytest.mark.parametrize("v,kept", [(20, 7), (2049, 200), (5000, 2700)])
 def test_xent_classes_masked_by_the_lowest_value_bf16(head, v, kept):
     masked_by_the_lowest_value(head, BF16, v, kept)
+
+
+@pytest.mark.parametrize("v,kept", [(20, 7), (2049, 200), (5000, 2700)])
+def test_xent_classes_masked_by_the_lowest_value_f32(head, v, kept):
+    masked_by_the_lowest_value(head, F32, v, kept)
