@@ -83,8 +83,7 @@ constexpr int kJoinWarps = 16;
 __device__ __forceinline__ float2 joined(float2 a, float2 b) {
   const float top = fmaxf(a.x, b.x);
   a.y = (a.x == top ? a.y : a.y * expf(a.x - top)) + (b.x == top ? b.y : b.y * expf(b.x - top));
-  // a NaN maximum (a product that gave up) stays
-  a.x = a.x != a.x || b.x != b.x ? NAN : top;
+  a.x = top;
   return a;
 }
 template <typename L>

@@ -347,6 +347,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_xent_mma(const __grid_constant_
           s = (add[0] + add[1]) + (add[2] + add[3]);
           m = top;
         }
+        // a half that gave up shows in the sum, whichever half it is
+        s = ok ? s : NAN;
         // the halves meet in the second warp's staging, which no stats tile uses
         const uint32_t meet = staging + (4 + quarter) * 4096 + buf * 256 + lane * 8;
         if (half) asm volatile("st.shared.v2.f32 [%0], {%1, %2};" ::"r"(meet), "f"(m), "f"(s) : "memory");
@@ -356,7 +358,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_xent_mma(const __grid_constant_
           asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(o.x), "=f"(o.y) : "r"(meet) : "memory");
           const float top = fmaxf(m, o.x), ref = top == -INFINITY ? 0.0f : top;
           s = s * exp_fast(m - ref) + o.y * exp_fast(o.x - ref);
-          p.part[(size_t)at.n * p.part_stride + row] = ok ? make_float2(top, s) : make_float2(NAN, NAN);
+          p.part[(size_t)at.n * p.part_stride + row] = make_float2(top, s);
         }
       } else if (job.kind == kJobGrad) {
         const bool in = row < job.n_rows;
