@@ -180,3 +180,24 @@ def test_xent_classes_masked_by_the_lowest_value_bf16(head, v, kept):
 @pytest.mark.parametrize("v,kept", [(20, 7), (2049, 200), (5000, 2700)])
 def test_xent_classes_masked_by_the_lowest_value_f32(head, v, kept):
     masked_by_the_lowest_value(head, F32, v, kept)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("size", [1e25, 3e30, 1e-25, 1e-30, 1e-37])
+def test_clip_squares_past_the_range_of_f32(head, dtype, size):
+    g = gen(6)
+    for sizes, common in (([5, 70001], size), ([200003, 3], 1e-3 * size), ([7] * 40, 0.0)):
+        t = [rand(g, s, dtype=dtype, by=common) for s in sizes]
+        t[0][3] = t[-1][1] = size
+        before = [a.clone() for a in t]
+        want = math.sqrt(sum(float(a.double().square().sum()) for a in t))
+        assert abs(float(head.grad_norm(t)) - want) <= 32 * U * want
+        max_norm = 0.5 * want
+        norm = head.clip_grad_norm(t, max_norm)
+        assert abs(float(norm) - want) <= 32 * U * want
+        by = min(1.0, max_norm / (want + 1e-6))
+        for a, b in zip(t, before):
+            w = b.double() * by
+            # the factor's own error, the output's rounding, and the smallest steps of either
+            bound = w.abs() * (UNIT[dtype] + 64 * U) + 2.0**-133 + b.double().abs() * 2.0**-148
+            assert ((a.double() - w).abs() <= bound).all()
