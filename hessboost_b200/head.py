@@ -8,7 +8,7 @@ entropy of a linear layer over the classes (any number of them, where
 ``multi:softmax`` grows a tree per class and stops at 64). These are its
 operators, each a forward and a backward call, and the clipping of its
 gradients; ``embed``, ``layer_norm`` and ``linear_xent`` are the same calls
-under autograd.
+under autograd, once: differentiating their gradients raises RuntimeError.
 
 All tensors are on one CUDA device; the kernels run on torch's current stream
 of it, nothing synchronises, and outputs are new contiguous tensors. A wrong
@@ -21,6 +21,7 @@ import ctypes
 import operator
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import HB_OK, HbError, lib
 
@@ -339,6 +340,8 @@ def clip_grad_norm(tensors, max_norm, *, out=None):
 
 
 # --------------------------------------------------------------- autograd
+# The backward calls are kernels without a graph of their own: a gradient that
+# is differentiated again (create_graph) raises.
 class _Embed(torch.autograd.Function):
     @staticmethod
     def forward(ctx, tokens, table, row_ptr, scale):
@@ -347,6 +350,7 @@ class _Embed(torch.autograd.Function):
         return embed_forward(tokens, table, row_ptr=row_ptr, scale=scale)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, grad):
         tokens, row_ptr = ctx.saved_tensors
         return None, embed_backward(grad, tokens, ctx.n_tokens, row_ptr=row_ptr, scale=ctx.scale), None, None
@@ -361,6 +365,7 @@ class _LayerNorm(torch.autograd.Function):
         return y
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dy):
         x, weight, mean, rstd = ctx.saved_tensors
         dx, dw, db = layer_norm_backward(dy, x, weight, mean, rstd, params=weight is not None or ctx.has_bias)
@@ -375,6 +380,7 @@ class _LinearXent(torch.autograd.Function):
         return loss
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dloss):
         dx, dw = linear_xent_backward(dloss, *ctx.saved_tensors)
         return dx, dw, None
