@@ -336,6 +336,8 @@ def clip_grad_norm(tensors, max_norm, *, out=None):
     ws, size = _workspace(L.hb_grad_norm_workspace, norm.device, dev, n)
     _check(L.hb_clip_grad_norm(dev, n, _address(ptrs), _address(outs), _address(sizes), _address(types), max_norm,
                                norm.data_ptr(), ws.data_ptr(), size, _stream(dev)), "hb_clip_grad_norm")
+    # written through addresses: a graph that has saved one of them is to notice
+    torch.autograd.graph.increment_version(tensors if out is None else out)
     return norm
 
 

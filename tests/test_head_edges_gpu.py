@@ -201,3 +201,27 @@ def test_clip_squares_past_the_range_of_f32(head, dtype, size):
             # the factor's own error, the output's rounding, and the smallest steps of either
             bound = w.abs() * (UNIT[dtype] + 64 * U) + 2.0**-133 + b.double().abs() * 2.0**-148
             assert ((a.double() - w).abs() <= bound).all()
+
+
+def test_clip_in_place_is_noticed_by_autograd(head):
+    # a tensor that a graph has saved changes under it: the graph says so instead of using the new values
+    a = torch.ones(50, device="cuda", requires_grad=True)
+    t = a * 3.0
+    y = (t * t).sum()
+    head.clip_grad_norm([t.detach()], 1.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+    t = a * 3.0
+    y = (t * t).sum()
+    head.clip_grad_norm([torch.ones(50, device="cuda")], 1.0, out=[t.detach()])
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+    # what is only read stays usable
+    t = a * 3.0
+    y = (t * t).sum()
+    head.grad_norm([t.detach()])
+    head.clip_grad_norm([t.detach()], 1.0, out=[torch.empty(50, device="cuda")])
+    y.backward()
+    assert (a.grad == 18).all()
+    with torch.inference_mode():
+        head.clip_grad_norm([torch.ones(3, device="cuda")], 1.0)
