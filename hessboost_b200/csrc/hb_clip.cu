@@ -16,6 +16,8 @@
 // adds the first one's sums itself.
 #include <algorithm>
 #include <cmath>
+#include <memory>
+#include <new>
 
 #include "hb_head.h"
 
@@ -263,6 +265,35 @@ hb_status check_tensors(int32_t n, const void* const* tensors, const uint64_t* s
   return HB_OK;
 }
 
+// No output may overlap another output, nor an input but its own, which it
+// then is: the chunks of a call run in no order, so an element that two of them
+// wrote, or one read and one wrote, would be scaled once or twice by chance.
+hb_status check_apart(int32_t n, const void* const* tensors, void* const* outs, const uint64_t* sizes, const int32_t* dtypes) {
+  struct Range {
+    uintptr_t begin, end;
+  };
+  if (!n) return HB_OK;
+  const std::unique_ptr<Range[]> ranges(new (std::nothrow) Range[n]);
+  if (!ranges) return fail(HB_REFUSED, "out of host memory");
+  const auto range = [&](int i, const void* p) {
+    const uintptr_t at = reinterpret_cast<uintptr_t>(p);
+    return Range{at, at + sizes[i] * size_of(dtypes[i])};
+  };
+  int count = 0;
+  for (int i = 0; i < n; ++i)
+    if (sizes[i]) ranges[count++] = range(i, outs[i]);
+  std::sort(ranges.get(), ranges.get() + count, [](const Range& a, const Range& b) { return a.begin < b.begin; });
+  for (int i = 1; i < count; ++i) HB_HEAD_REQUIRE(ranges[i].begin >= ranges[i - 1].end, "two outputs overlap");
+  for (int i = 0; i < n; ++i) {
+    if (!sizes[i] || tensors[i] == outs[i]) continue;  // its own output, which is apart from the others
+    const Range r = range(i, tensors[i]);
+    // the last output that begins before the input's end: those before it end before it begins
+    const Range* after = std::lower_bound(ranges.get(), ranges.get() + count, r.end, [](const Range& a, uintptr_t v) { return a.begin < v; });
+    HB_HEAD_REQUIRE(after == ranges.get() || after[-1].end <= r.begin, "an output overlaps an input that is not its own");
+  }
+  return HB_OK;
+}
+
 // Chunks of a tensor: of its vectors, one at least for its other elements.
 uint32_t chunks_of(uint64_t n, int32_t dtype) {
   return (uint32_t)std::max<uint64_t>(1, (n * size_of(dtype) / 16 + kChunk - 1) / kChunk);
@@ -347,6 +378,7 @@ hb_status hb_clip_grad_norm(int32_t device, int32_t n_tensors, const void* const
   HB_HEAD_REQUIRE(outs || !n_tensors, "outs is NULL");
   for (int i = 0; i < n_tensors; ++i)
     HB_HEAD_REQUIRE((outs[i] || !sizes[i]) && aligned(outs[i], size_of(dtypes[i])), "an output is NULL or not aligned to its type");
+  if (hb_status st = check_apart(n_tensors, tensors, outs, sizes, dtypes)) return st;
   const int sms = sm_count(device);
   HB_HEAD_REQUIRE(workspace && aligned(workspace, 8) && workspace_bytes >= 8 * most_sums(n_tensors, sms),
                   "workspace is too small or not 8-byte aligned");

@@ -319,8 +319,8 @@ def grad_norm(tensors):
 
 def clip_grad_norm(tensors, max_norm, *, out=None):
     """The tensors' norm (as grad_norm), after scaling each tensor by min(1, max_norm / (norm + 1e-6)): in place, or
-    into `out`, a list of as many contiguous tensors of the same sizes and types. A norm that is not finite passes into
-    the results through that factor."""
+    into `out`, a list of as many contiguous tensors of the same sizes and types. Outputs that overlap (a tensor listed
+    twice, in place) are refused. A norm that is not finite passes into the results through that factor."""
     tensors = list(tensors)
     _need(max_norm >= 0, "max_norm must be >= 0")
     n, ptrs, sizes, types, dev = _tensor_list(tensors)

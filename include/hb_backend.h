@@ -526,8 +526,10 @@ hb_status hb_grad_norm(int32_t device, int32_t n_tensors, const void* const* ten
                        const int32_t* dtypes, float* norm, void* workspace, uint64_t workspace_bytes,
                        void* stream);
 /* hb_grad_norm, then outs[i] = tensors[i] * min(1, max_norm / (*norm +
- * 1e-6)), each of its tensor's type; outs[i] may be tensors[i]. A norm that
- * is not finite shows in *norm and passes into the outputs. */
+ * 1e-6)), each of its tensor's type; outs[i] may be tensors[i]. Outputs that
+ * overlap one another (a tensor listed twice, in place) or another tensor's
+ * input are refused. A norm that is not finite shows in *norm and passes into
+ * the outputs. */
 hb_status hb_clip_grad_norm(int32_t device, int32_t n_tensors, const void* const* tensors, void* const* outs,
                             const uint64_t* sizes, const int32_t* dtypes, float max_norm, float* norm,
                             void* workspace, uint64_t workspace_bytes, void* stream);

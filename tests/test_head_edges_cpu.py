@@ -1,7 +1,11 @@
 """The embedding head's autograd forms and refusals, where no GPU is needed: the calls that would launch kernels are
 replaced by plain formulas, or are refused before they touch the device."""
 
+import ctypes
+
 import pytest
+
+import hessboost_b200 as H
 
 torch = pytest.importorskip("torch")
 
@@ -69,3 +73,37 @@ def test_gradients_are_differentiable_once(monkeypatch, name):
     penalty = sum(t.square().sum() for t in grads) + sum(t.square().sum() for t in p)
     with pytest.raises(RuntimeError, match="once_differentiable"):
         penalty.backward()
+
+
+P = 0x10000  # addresses that no call reads
+
+
+@pytest.mark.parametrize("ins,outs,refused", [
+    ([0, 0], [0, 0], "two outputs overlap"),                       # a tensor listed twice, in place
+    ([0, 40], [0, 20], "two outputs overlap"),
+    ([400, 800], [60, 56], "two outputs overlap"),
+    ([0, 400], [4, 800], "not its own"),                           # an output one element off its input
+    ([0, 400], [800, 20], "not its own"),                          # over another tensor's input
+    ([400, 0], [20, 800], "not its own"),
+    ([0, 40], [0, 40], None),                                      # in place, side by side
+    ([40, 0], [40, 0], None),
+    ([0, 0], [80, 40], None),                                      # one input twice, apart from the outputs
+    ([0, 20], [120, 160], None),
+    ([0, 80], [0, 40], None),                                      # one in place, one not
+])
+def test_clip_refuses_outputs_that_overlap(ins, outs, refused):
+    # two tensors of 10 f32: the chunks of a call run in no order, so an element written twice would be scaled by chance
+    L = H.lib()
+    a, b = (ctypes.c_void_p * 2)(*[P + i for i in ins]), (ctypes.c_void_p * 2)(*[P + o for o in outs])
+    sizes, types = (ctypes.c_uint64 * 2)(10, 10), (ctypes.c_int32 * 2)(0, 0)
+    # a call that passes is refused for its workspace, the next thing looked at
+    assert L.hb_clip_grad_norm(0, 2, a, b, sizes, types, 1.0, P, None, 0, None) == H.HB_INVALID_ARGUMENT
+    assert (refused or "workspace") in L.hb_head_last_error().decode()
+
+
+def test_clip_of_empty_tensors_overlaps_nothing():
+    L = H.lib()
+    a, types = (ctypes.c_void_p * 2)(P, P), (ctypes.c_int32 * 2)(0, 0)
+    for sizes in ((10, 0), (0, 10), (0, 0)):
+        assert L.hb_clip_grad_norm(0, 2, a, a, (ctypes.c_uint64 * 2)(*sizes), types, 1.0, P, None, 0, None) == H.HB_INVALID_ARGUMENT
+        assert "workspace" in L.hb_head_last_error().decode()
