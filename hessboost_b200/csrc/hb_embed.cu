@@ -8,12 +8,13 @@
 // cells is 0. Sums are f32 in a fixed order, rounded once to the table's
 // type, so results do not change from run to run.
 //
-// Both directions move one row of `width` elements a cell through the L2
-// cache, which bounds them (the tables and gradients of a head fit there), as
-// long as little else is issued for a cell: the lanes of a row load 8 tokens
-// together and pass them round, a row's address is one multiply-add, and two
-// f32 are added at a time. 5.2M cells of 128 bf16 took 298 us forward with
-// every lane working out its own addresses.
+// Both directions move one row of `width` elements a cell through the L2 cache
+// (the tables and gradients of a head fit there) and are bound by what is issued
+// for a cell and by waiting for its row: 5.2M cells of 128 bf16 take 135 us
+// forward, 11 TB/s of the L2 cache (43% of its rate) with an instruction issued
+// in 65% of the cycles. So the lanes of a row load 8 tokens together and pass
+// them round, a row's address is one multiply-add, and two f32 are added at a
+// time; with every lane working out its own addresses it took 298 us.
 //
 // The gradient sorts the cells by token (a stable radix sort of (token, row)
 // pairs, digits of at most 10 bits) and sums the sorted cells' rows in chunks

@@ -42,7 +42,11 @@ constexpr int kGroupThreads = 256;
 // Who holds a row: a group of lanes, a CTA of which there are two an SM (the
 // forward pass alone: 8,191 x 4,097 f32 take it 50 us, 78 with one; the
 // backward pass's column sums then spill, 116 us for 96), or a larger one. The
-// most threads of each, by the registers of 16 elements a thread.
+// most threads of each, by the registers of 16 elements a thread: two CTAs end
+// at 4,608 columns. From 600 to there, 67M elements, they are 6 to 45% faster
+// in bf16 (as fast at 4,608) and 2 to 30% off 16-byte boundaries, where f32 of
+// 600 columns is 6% slower; f32 vectors are 22% faster at 600 and 1 to 9%
+// slower from 1,000.
 enum Holder { kByGroup, kBySmall, kByLarge };
 constexpr int max_threads(int holder) { return holder == kByGroup ? kGroupThreads : holder == kBySmall ? 288 : 512; }
 constexpr int kLoopThreads = 512;

@@ -25,9 +25,10 @@ struct MmaOut {
 // Pieces (bf16) of G. One, rounded as dx and dw are, would not do for bf16
 // layers either: a row of G sums to 0 over the classes, so what their weights
 // share cancels in dx, but the roundings of G times it do not. Weights of 8
-// with a spread of 0.25 then leave 5% of dx; with two pieces it is 2^-8 of
+// with a spread of 0.25 then leave 6% of dx; with two pieces it is 2^-8 of
 // that, and bf16 weights have no finer spread. Both products are done twice
-// for it: 8,192 x 1,024 rows with 50,021 classes take 4.3 ms, 2.6 with one.
+// for it: 8,192 x 1,024 rows with 50,021 classes take 4.5 ms pass after pass,
+// 3.0 with one.
 constexpr int kGradPlanesBf16 = 2, kGradPlanesF32 = 3;
 constexpr int kMmaDepth = 2;  // blocks of 64 of k in a stage
 // Stages of z's k that are summed in the tensor cores, and whether there are more.

@@ -6,19 +6,24 @@
 //   dx     G w      (k: the piece's classes)
 //   dw     G^T x    (k: the rows)
 //
-// One persistent kernel runs a list of such jobs: tile t of the list goes to
-// CTA t mod grid. A CTA's warp 0 feeds 64-deep steps of both operands
-// through a ring of shared-memory stages by TMA, warp 1 issues the MMAs of a
-// 128 x n tile (n <= 256) into one of two TMEM accumulators, and warps 4 to 7
-// work the other one off. Operands are read as they lie, whether k or their
-// own rows run along memory, so G is written once, row by row, and read by dx
-// (k along memory) and by dw (its classes along memory).
+// One persistent kernel runs a list of such jobs, whose tiles share_out deals to
+// the CTAs, or pairs of them, in runs of about equal work. A CTA's warp 0 feeds
+// 128-deep stages of both operands through a ring in shared memory by TMA, warp
+// 1 issues the MMAs of a 128 x n tile (a pair's is 256 x n, n <= 256) into one
+// of two TMEM accumulators, and warps 4 to 11 work the other one off. Operands
+// are read as they lie, whether k or their own rows run along memory, so G is
+// written once, row by row, and read by dx (k along memory) and by dw (its
+// classes along memory).
 //
 // Every operand is seen as [plane][block of 64 columns][row][64 columns], so
 // that one copy brings a CTA's whole share of an operand for a stage: with
 // 64 x 64 copies (8 KiB each) the copies themselves were the limit, 990
-// TFLOP/s on 8,192 x 1,024 x 50,021 against 1,330 with 128 x 64 ones. It takes
-// rows of whole blocks: columns past an operand's width are zeros.
+// TFLOP/s on 8,192 x 1,024 x 50,021 against 1,330 with 128 x 64 ones, both
+// before the clocks fall. Bound by the tensor cores and then by power: the
+// logits of that size take 599 us cold (1.40 PFLOP/s, tensor pipe 77% busy), a
+// piece's dx and dw with the next one's G 317 (82%); the whole call's 5.0
+// TFLOP, pass after pass, 4.5 ms (1.1 PFLOP/s at the clocks of the power cap).
+// It takes rows of whole blocks: columns past an operand's width are zeros.
 //
 // f32 operands are three bf16 pieces (v = p0 + p1 + p2, each the rounding of
 // what the ones before leave), and a product is the six products of pieces

@@ -495,9 +495,12 @@ hb_status hb_layer_norm_backward(int32_t device, const void* dy, uint64_t dy_str
  * exp(z[n])), z = x w^T: x n_rows x width, w n_classes x width, both f32 or
  * both bf16. The logits are never kept. A label outside [0, n_classes) is a
  * row without a label: its loss is 0 (its lse is still written). bf16 rows
- * that start on 16-byte boundaries (address and stride) are read as they
- * lie, others are laid out in the workspace first: its size goes by x and w
- * too. */
+ * that start on 16-byte boundaries (address and stride) and whose width is a
+ * multiple of 64 are read as they lie, others are laid out in the workspace
+ * first: its size goes by x and w too. A loss is never below 0. A class is
+ * masked by the type's lowest value in a column of w that meets ones in x
+ * (an infinity there does not do: it makes NaN of that column of dx, and in
+ * f32, past a few classes, of every logit it meets). */
 hb_status hb_linear_xent_forward_workspace(int32_t device, const void* x, uint64_t x_stride, const void* w,
                                           uint64_t w_stride, int32_t dtype, uint64_t n_rows, uint32_t width,
                                           uint64_t n_classes, uint64_t* bytes);
@@ -507,8 +510,9 @@ hb_status hb_linear_xent_forward(int32_t device, const void* x, uint64_t x_strid
                                  float* lse, void* workspace, uint64_t workspace_bytes, void* stream);
 /* dx and dw (contiguous) of sum over n of dloss[n * dloss_stride] loss[n]
  * (dloss_stride 0: one factor for every row); lse from the forward pass. The
- * logits are computed again, a piece of the classes at a time. Rows without
- * a label get 0 and add nothing. */
+ * logits are computed again, a piece of the classes at a time, and exp(z -
+ * lse) - [class = label] times dloss is held to 16 bits of mantissa for bf16
+ * layers, 24 for f32. Rows without a label get 0 and add nothing. */
 hb_status hb_linear_xent_backward_workspace(int32_t device, const void* x, uint64_t x_stride, const void* w,
                                           uint64_t w_stride, int32_t dtype, uint64_t n_rows, uint32_t width,
                                           uint64_t n_classes, uint64_t* bytes);
