@@ -19,9 +19,9 @@ namespace {
 
 // Elements of G's pieces held at a time (160 MiB in bf16): with half as many,
 // twice the launches, 8,192 x 1,024 bf16 rows with 50,021 classes take 4.7 ms
-// for 4.3 (a burst of passes), 2,048 x 2,048 with 32,000 classes 1.23 for 1.30. In f32 as many
-// would make 4,099 x 257 rows with 12,289 classes 791 us for 813, but the
-// chunks of rows, and with them the parts that dw is summed in, twice as many.
+// for 4.3 (a burst of passes), 2,048 x 2,048 with 32,000 classes 1.23 for
+// 1.30. In f32 as many would take 3% off 4,099 x 257 rows with 12,289 classes
+// and double the accumulators of dx and dw.
 constexpr int64_t kGradElementsBf16 = 80ll << 20, kGradElementsF32 = 40ll << 20;
 constexpr uint64_t kPartBytes = 64ull << 20;   // of the stats' parts held at a time
 constexpr int kFinishThreads = 256;
@@ -194,14 +194,16 @@ int last_cols(uint64_t cols, int n, bool pair) {
 }
 // Parts of k: enough tiles for the workers, at least 4 steps of 64 each, and
 // none longer than its type's sums may be, since the tensor cores' own sums
-// round towards zero. In f32 that is 1,024: dw of 131,072 to 600,000 rows is
-// then 15 to 23 U off (U = 2^-24; plain f32 sums 4 to 11), whatever its terms'
-// signs; with parts of 2,600 it was 50 to 99 U, of 8,100 140 to 500 U. In bf16
-// it is 32,768, some 2^-12 of the result.
+// round towards zero: 0.7 U of what is summed so far on average (U = 2^-24) in
+// each step of 16. In f32 that is 512: dw of 131,072 to 600,000 rows is then
+// 6 to 16 U off (plain f32 sums 3 to 11) where parts of 1,024 made it 15 to 23,
+// of 2,600 50 to 99, of 8,100 140 to 500, and dx over 16,918 classes 13 U for
+// 17 to 22 (plain 12). (4,099 x 257 rows with 12,289 classes: 850 us, 816 with
+// parts of 1,024, 964 of 256.) In bf16 it is 32,768, some 2^-12 of the result.
 int k_splits(uint64_t tiles, int k_blocks, int workers, int planes) {
   const int want = tiles >= (uint64_t)workers ? 1 : (int)((workers + tiles - 1) / tiles);
   const int by_tiles = std::max(1, std::min(want, k_blocks * kMmaDepth / 4));
-  const int longest = (planes == 1 ? 32768 : 1024) / (64 * kMmaDepth);  // in k_blocks
+  const int longest = (planes == 1 ? 32768 : 512) / (64 * kMmaDepth);  // in k_blocks
   return std::max(by_tiles, (k_blocks + longest - 1) / longest);
 }
 
@@ -243,8 +245,13 @@ Backward backward_plan(const Sizes& z, int32_t dtype, const void* x, uint64_t x_
   b.x = operand_of(z, dtype, x, x_stride, z.n_rows, true);
   b.w = operand_of(z, dtype, w, w_stride, z.n_classes, false);
   const uint64_t most = (uint64_t)(z.planes == 1 ? kGradElementsBf16 : kGradElementsF32) / z.g_planes;
-  const uint64_t least = 2048;  // classes of a piece, where there are as many
-  b.chunk = std::min(z.n_rows, std::max<uint64_t>(most / std::min(z.n_classes, least) / 256 * 256, 256));
+  // `least`: classes of a piece, where there are as many
+  const auto chunk_of = [&](uint64_t least) { return std::min(z.n_rows, std::max<uint64_t>(most / std::min(z.n_classes, least) / 256 * 256, 256)); };
+  b.chunk = chunk_of(2048);
+  // several chunks of rows keep dw's accumulators of all the classes between
+  // them, in f32 one for each 512 rows: chunks of about 2,048 (8,192 x 1,024
+  // f32 rows with 20,000 classes: 711 MB of workspace for 1,080, 8.6 ms for 8.8)
+  if (z.planes > 1 && b.chunk < z.n_rows) b.chunk = chunk_of(most / 2048);
   b.chunks = (z.n_rows + b.chunk - 1) / b.chunk;
   b.chunk = std::min(b.chunk, round_up((z.n_rows + b.chunks - 1) / b.chunks, 256));
   b.piece = std::min(z.n_classes, std::max<uint64_t>(most / b.chunk / 256 * 256, 256));

@@ -99,6 +99,22 @@ def test_xent_long_sums_in_f32(head, n, d, v, one_sign):
     assert off(dw, xent64(x, w, labels, dl)["dw"]) <= 128 * U
 
 
+@pytest.mark.parametrize("n,d,v", [(33, 1970, 16918), (300000, 1024, 40), (600000, 600, 20), (9000, 72, 5000)])
+def test_xent_f32_gradients_are_as_near_as_f32_sums(head, n, d, v):
+    # a part of 512 has 32 steps, each off by half a unit in the last place of what is summed so far: 0.72 U on average
+    # over its mantissas. Of terms of either sign, what is summed after i steps is about sqrt(i / 32) of the part:
+    # 0.72 U x 21.6 = 15.5 U, always towards zero, so of the whole sum too. 2.5 U for p and the output's rounding
+    g = gen(n + 1)
+    x, w = rand(g, n, d), rand(g, v, d, by=d**-0.5)
+    labels = torch.randint(v, (n,), generator=g, device="cuda")
+    dl = (0.5 + torch.rand(n, generator=g, device="cuda")) / n
+    _, lse = head.linear_xent_forward(x, w, labels)
+    dx, dw = head.linear_xent_backward(dl, x, w, labels, lse)
+    r = xent64(x, w, labels, dl)
+    assert off(dx, r["dx"]) <= 18 * U
+    assert off(dw, r["dw"]) <= 18 * U
+
+
 @pytest.mark.parametrize("n,d,v", [(130, 2056, 700), (512, 4096, 3000), (300, 16384, 1000), (3000, 4100, 2600)])
 def test_xent_logits_of_wide_bf16_rows(head, n, d, v):
     # the loss is f32: logits of about 1 in parts of 2,048, 128 steps of 16 each off by 2 U of what is summed so far (half
